@@ -174,6 +174,22 @@ class BfsrChainConv(C.Structure):
     ]
 
 
+class BfsrListArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_void_p), ("chunks", C.c_void_p),
+        ("n", C.c_int), ("count", C.c_int), ("chunk", C.c_int), ("max", C.c_int),
+        ("other", C.c_void_p), ("work", C.c_void_p), ("norm", C.c_void_p),
+    ]
+
+
+class BfsrAdamArgs(C.Structure):
+    _fields_ = [
+        ("lr", C.c_double), ("lr_at", C.c_void_p),
+        ("beta1", C.c_double), ("beta2", C.c_double), ("weight_decay", C.c_double), ("eps", C.c_float),
+        ("decoupled", C.c_int), ("max_norm", C.c_float), ("given_norm", C.c_void_p), ("skip_nonfinite", C.c_int),
+    ]
+
+
 # every symbol include/bfsr_hip.h declares: name -> (restype, argtypes)
 _LL, _I, _F, _VP = C.c_longlong, C.c_int, C.c_float, C.c_void_p
 SYMBOLS = {
@@ -269,6 +285,13 @@ SYMBOLS = {
     "bfsr_to_uint8": (_I, [_VP, _LL, _VP, _I, _LL, _VP]),
     "bfsr_channel_range_scratch": (_LL, [_I, _I]),
     "bfsr_channel_range_check": (_I, [_VP, _LL, _I, _I, _I, _I, _F, _F, _F, _VP, _VP, _VP, _VP]),
+    "bfsr_list_chunk": (_I, [_LL]),
+    "bfsr_list_work": (_LL, [_I]),
+    "bfsr_list_write": (_I, [_VP, _I, _VP, _VP, _I, _I, _VP, _VP, _VP]),
+    "bfsr_pointer_write": (_I, [_VP, _I, _VP, _VP]),
+    "bfsr_grad_norm": (_I, [C.POINTER(BfsrListArgs), _VP]),
+    "bfsr_clip_grads": (_I, [C.POINTER(BfsrListArgs), _F, _VP]),
+    "bfsr_adam_step": (_I, [C.POINTER(BfsrListArgs), C.POINTER(BfsrAdamArgs), _VP]),
     "bfsr_conv2d_direct": (_I, [_VP, _LL, _VP, _VP, _VP, _LL, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _VP]),
 }
 

@@ -10,12 +10,15 @@ logging are outside the accelerated path."""
 import torch
 import torch.nn.functional as F
 
+from ..optim import clip_grad_norm
 
-def train_step(prior_model, linf_model, batch, optimizer=None, latent_weight=1.0, image_weight=0.0, feat_fn=None, patch=True):
+
+def train_step(prior_model, linf_model, batch, optimizer=None, latent_weight=1.0, image_weight=0.0, feat_fn=None, patch=True, max_grad_norm=None):
     """One iteration of train.py:118-160 on a batch dict (inp, gt, coord, cell, gt_lr_up, gt_patch | gt_pixel, [interpolate_coord]),
     tensors in the reference's normalisation (inp, gt in [0,1]; sub = div = 0.5).  `image_weight` / `feat_fn` are train.py's
     `vgg_weight` / `vgg`.  Returns dict(loss, latent, image) of floats;
-    with `optimizer` the step is applied."""
+    with `optimizer` the step is applied.  `max_grad_norm`: the latent module's gradients are clipped by their global norm first (optim.clip_grad_norm on the
+    model's kernels), and the dict gets `grad_norm`, the norm before.  `bfsr_amd.optim.Adam` is the reference's optimizer on the kernels."""
     eng = linf_model.engine()
     d = eng.ops.to_device
     inp = (d(batch["inp"]) - 0.5) / 0.5                                           # train.py:122
@@ -58,6 +61,11 @@ def train_step(prior_model, linf_model, batch, optimizer=None, latent_weight=1.0
         if optimizer is not None:
             optimizer.zero_grad()
         loss.backward()
+        if max_grad_norm is not None:
+            norm = clip_grad_norm(prior_model.parameters(), max_grad_norm, ops=eng.ops)
         if optimizer is not None:
             optimizer.step()
-    return dict(loss=float(loss.detach()), latent=float(latent_l.detach()), image=float(image_l.detach()))
+    out = dict(loss=float(loss.detach()), latent=float(latent_l.detach()), image=float(image_l.detach()))
+    if max_grad_norm is not None:
+        out["grad_norm"] = float(norm)
+    return out

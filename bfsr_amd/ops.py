@@ -5,9 +5,12 @@ PyTorch is plumbing here (device memory, streams); all arithmetic on the hot pat
 libbfsr_hip.so.  `HipOps` is the only ops backend of the product; tests may substitute a CPU
 test double with the same interface to exercise the host-side schedule without a GPU.
 """
+import contextlib
 import ctypes as C
+import math
 import os
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -78,6 +81,235 @@ class ConvChain(object):
             "conv_chain_launch")
 
 
+# ---- lists of tensors (tensor_list.hip) ----------------------------------------------------------
+LIST_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _order(t):
+    """The strides of the axes that have any: two tensors of one shape with the same ones hold their elements in the same order."""
+    return tuple(s for s, n in zip(t.stride(), t.shape) if n != 1) if t.numel() else ()
+
+
+def _dense(t):
+    """Whether the elements fill one piece of memory, in any order of the axes, each with a place of its own."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if s != expect:
+            return False
+        expect *= n
+    return True
+
+
+def list_column(tensors, device, what, types=LIST_TYPES, like=None):
+    """`tensors` as a list of aliases without a graph, every one checked: dense memory of one of `types` on `device`; shapes and orders of `like`, tensor by tensor."""
+    if isinstance(tensors, torch.Tensor):
+        raise TypeError("%s: need a list of tensors, got one tensor" % what)
+    got = list(tensors)
+    if like is not None and len(got) != len(like):
+        raise ValueError("%s: %d tensors, need %d" % (what, len(got), len(like)))
+    for k, t in enumerate(got):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("%s[%d]: need a tensor, got %s" % (what, k, type(t).__name__))
+        if t.layout != torch.strided or t.dtype not in types or t.device != device:
+            raise ValueError("%s[%d]: need a strided tensor of %s on %s, got %s, %s on %s" % (
+                what, k, " / ".join(str(d)[6:] for d in types), device, t.layout, t.dtype, t.device))
+        if t.is_neg() or not _dense(t):
+            raise ValueError("%s[%d]: not dense memory (shape %s, strides %s)" % (what, k, tuple(t.shape), t.stride()))
+        if like is not None and (t.shape != like[k].shape or _order(t) != _order(like[k])):
+            raise ValueError("%s[%d]: shape %s, strides %s do not go with shape %s, strides %s" % (
+                what, k, tuple(t.shape), t.stride(), tuple(like[k].shape), like[k].stride()))
+    return [t.detach() for t in got]
+
+
+class Spans(object):
+    """The pieces of memory that tensors take, sorted; they may not overlap."""
+
+    def __init__(self, tensors, what):
+        live = [(t.data_ptr(), t.numel() * t.element_size()) for t in tensors if t.numel()]
+        a = np.array(live, dtype=np.int64).reshape(-1, 2)
+        a = a[np.argsort(a[:, 0], kind="stable")]
+        self.start, self.end = a[:, 0], a[:, 0] + a[:, 1]
+        if (self.start[1:] < self.end[:-1]).any():
+            raise ValueError("%s: two of the tensors that are written overlap (or one is there twice)" % what)
+
+    def meet(self, tensors):
+        """Whether one of `tensors` overlaps one of these."""
+        live = [(t.data_ptr(), t.numel() * t.element_size()) for t in tensors if t.numel()]
+        if not live or not self.start.size:
+            return False
+        a = np.array(live, dtype=np.int64)
+        k = np.searchsorted(self.end, a[:, 0], side="right")           # the first piece that ends behind the tensor's start
+        near = np.minimum(k, self.start.size - 1)
+        return bool(((k < self.start.size) & (self.start[near] < a[:, 0] + a[:, 1])).any())
+
+
+class ListTable(object):
+    """The device table of a list of tensors (HipOps.tensor_list, HipOps.adam).  It names the memory that the tensors had when it was made, and holds on to it."""
+
+    def __init__(self, ops, cols, types, once):
+        self.ops, self.n, self.once = ops, len(cols[0]), once
+        self.sizes = [t.numel() for t in cols[0]]
+        self.chunk = ops.lib.bfsr_list_chunk(sum(self.sizes))
+        self.count = sum(-(-s // self.chunk) for s in self.sizes)
+        if self.count >= 1 << 24:
+            raise ValueError("tensor list: %d elements are too many for one list" % sum(self.sizes))
+        self.stream, self.table = None, None
+        if not self.n:
+            return
+        dev = ops._index_device()
+        with torch.cuda.device(dev):
+            if not once and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("tensor list: make it before the capture begins (its table is written once, not at every replay)")
+            stream = torch.cuda.current_stream(dev)
+            self.stream = stream.cuda_stream
+            self.table = torch.empty(self.n * 8 + max(self.count, 1), dtype=torch.int64, device=dev)
+            n = self.n
+            held = [(C.c_void_p * n)(*[t.data_ptr() for t in c]) for c in cols]
+            ptrs = (C.c_void_p * len(cols))(*[C.addressof(h) for h in held])
+            _lib.check(ops.lib.bfsr_list_write(ptrs, len(cols), (C.c_longlong * n)(*self.sizes), (C.c_int * n)(*types), n, self.chunk,
+                                               self.table.data_ptr(), self.table.data_ptr() + 64 * n, C.c_void_p(self.stream)), "list_write")
+            if not once:
+                stream.synchronize()               # from here on the table may be read on any stream
+
+    def args(self, ops, norm_type, norm):
+        """The C arguments of one call on the current stream, and that stream."""
+        stream = torch.cuda.current_stream(ops._index_device())
+        if self.once:
+            if stream.cuda_stream != self.stream:
+                raise RuntimeError("tensor list: one made with once=True belongs to the stream it was made on")
+        else:
+            if stream.cuda_stream != self.stream:
+                self.table.record_stream(stream)
+            if torch.cuda.is_current_stream_capturing():
+                ops._captured_tables.append(self.table)      # a graph reads it at every replay, whatever becomes of the list
+        a = _lib.BfsrListArgs()
+        a.rows = self.table.data_ptr()
+        a.chunks = a.rows + 64 * self.n
+        a.n, a.count, a.chunk, a.max = self.n, self.count, self.chunk, int(norm_type == math.inf)
+        work = torch.empty(ops.lib.bfsr_list_work(self.n) // 8, dtype=torch.float64, device=self.table.device)
+        a.work = work.data_ptr()
+        if norm is not None:
+            a.norm = norm.data_ptr()
+        return a, stream, work
+
+
+def _norm_type(v):
+    v = math.inf if v == "inf" else float(v)
+    if v not in (2.0, math.inf):
+        raise ValueError("norm_type: 2 or inf, got %r" % v)
+    return v
+
+
+def _at_least_0(v, what, below=math.inf):
+    v = float(v)
+    if not 0.0 <= v <= below or (below == 1.0 and v == 1.0):
+        raise ValueError("%s: %r is out of range" % (what, v))
+    return v
+
+
+def _one_float(t, device, what):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
+        raise ValueError("%s: need a tensor of one float32 on %s" % (what, device))
+    return t
+
+
+class TensorList(ListTable):
+    """A list of tensors for grad_norm and clip_grads (HipOps.tensor_list)."""
+
+    def __init__(self, ops, tensors, out=None, once=False):
+        dev = ops._index_device()
+        self.tensors = list_column(tensors, dev, "tensor_list")
+        self.out = None
+        if out is not None:
+            self.out = list_column(out, dev, "tensor_list.out", like=self.tensors)
+            if any(a.dtype != b.dtype for a, b in zip(self.tensors, self.out)):
+                raise ValueError("tensor_list.out: need the types of the tensors")
+        if Spans(self.tensors if out is None else self.out, "tensor_list").meet(self.tensors if out is not None else []):
+            raise ValueError("tensor_list.out: overlaps the tensors (leave `out` away to write in place)")
+        self.written = [t for t in (self.tensors if out is None else self.out) if not t.is_inference()]
+        super().__init__(ops, [self.tensors] if out is None else [self.tensors, self.out], [LIST_TYPES[t.dtype] for t in self.tensors], once)
+
+
+class AdamPlan(ListTable):
+    """Adam's update of a list of parameters (HipOps.adam)."""
+
+    def __init__(self, ops, params, grads, exp_avg, exp_avg_sq, step):
+        dev, f32 = ops._index_device(), {torch.float32: 0}
+        self.params = list_column(params, dev, "adam.params")
+        if not self.params:
+            raise ValueError("adam: the list of parameters is empty")
+        self.grads = None if grads is None else list_column(grads, dev, "adam.grads", like=self.params)
+        self.grad_types = [t.dtype for t in (self.grads or self.params)]
+        self.exp_avg = list_column(exp_avg, dev, "adam.exp_avg", f32, like=self.params)
+        self.exp_avg_sq = list_column(exp_avg_sq, dev, "adam.exp_avg_sq", f32, like=self.params)
+        if isinstance(step, torch.Tensor):
+            if step.dim() != 1:
+                raise ValueError("adam.step: need a 1-d tensor, or a list of tensors of one float32")
+            step = step.unbind()
+        self.step = [_one_float(t, dev, "adam.step").detach() for t in step]
+        if len(self.step) != len(self.params):
+            raise ValueError("adam.step: %d counts for %d parameters" % (len(self.step), len(self.params)))
+        self.spans = Spans(self.params + self.exp_avg + self.exp_avg_sq + self.step, "adam")
+        if self.spans.meet(self.grads or []):
+            raise ValueError("adam.grads: overlap what the update writes")
+        self.written = [t for t in self.params if not t.is_inference()]
+        super().__init__(ops, [self.params, self.grads or self.params, self.exp_avg, self.exp_avg_sq, self.step],
+                         [LIST_TYPES[p.dtype] | LIST_TYPES[g] << 4 for p, g in zip(self.params, self.grad_types)], False)
+
+    def run(self, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled=False, max_norm=None, norm_type=2.0, grad_norm=None, skip_nonfinite=False, grads=None):
+        """One step: the counts go up by one, moments and parameters are updated in place.  Nothing waits for the device; may be captured.
+
+        lr                a number, or a tensor of one float32 on the device, read at the time of the update (a captured graph then follows a schedule)
+        weight_decay      added to the gradient as weight_decay * p; `decoupled`: taken off the parameter as lr * weight_decay * p
+        max_norm          gradients count as if clip_grads(max_norm, norm_type) had run before; they stay as they are in memory
+        grad_norm         the norm to clip by (a tensor of one float32), where it is not this list's own: of several lists, or over ranks
+        skip_nonfinite    where the norm is infinite or NaN, nothing changes, step counts included
+        grads             the gradients of this step, where the plan has none or they stand elsewhere than its own (shapes and orders of the axes of the
+                          parameters, types of the plan's gradients)
+
+        Returns the norm before clipping (0-d, on the device) with max_norm or skip_nonfinite, None otherwise."""
+        ops = self.ops
+        dev = ops._index_device()
+        h = _lib.BfsrAdamArgs()
+        if isinstance(lr, torch.Tensor):
+            h.lr_at = _one_float(lr, dev, "adam.lr").data_ptr()
+        else:
+            h.lr = _at_least_0(lr, "adam.lr")
+        h.beta1, h.beta2 = (_at_least_0(b, "adam.betas", 1.0) for b in betas)
+        h.eps, h.weight_decay = _at_least_0(eps, "adam.eps"), _at_least_0(weight_decay, "adam.weight_decay")
+        h.decoupled, h.skip_nonfinite = int(bool(decoupled)), int(bool(skip_nonfinite))
+        h.max_norm = -1.0 if max_norm is None else _at_least_0(max_norm, "adam.max_norm")
+        norm_type = _norm_type(norm_type)
+        norm = None
+        if max_norm is not None or skip_nonfinite:
+            norm = torch.empty((), dtype=torch.float32, device=dev)
+            if grad_norm is not None:
+                h.given_norm = _one_float(grad_norm, dev, "adam.grad_norm").data_ptr()
+        elif grad_norm is not None:
+            raise ValueError("adam.grad_norm: goes with max_norm or skip_nonfinite")
+        if grads is None:
+            if self.grads is None:
+                raise ValueError("adam.grads: the plan was made without gradients, so run() needs them")
+        else:
+            grads = list_column(grads, dev, "adam.grads", like=self.params)
+            if any(g.dtype != t for g, t in zip(grads, self.grad_types)):
+                raise ValueError("adam.grads: need the types of the plan's gradients")
+            if self.spans.meet(grads):
+                raise ValueError("adam.grads: overlap what the update writes")
+        with ops._on_device():
+            a, stream, work = self.args(ops, norm_type, norm)
+            st = C.c_void_p(stream.cuda_stream)
+            if grads is not None:
+                other = torch.empty(self.n, dtype=torch.int64, device=dev)
+                _lib.check(ops.lib.bfsr_pointer_write((C.c_void_p * self.n)(*[g.data_ptr() for g in grads]), self.n, other.data_ptr(), st), "pointer_write")
+                a.other = other.data_ptr()
+            _lib.check(ops._launch(("adam_step", self.n, self.count), lambda: ops.lib.bfsr_adam_step(C.byref(a), C.byref(h), st)), "adam_step")
+        torch.autograd.graph.increment_version(self.written)
+        return norm
+
+
 class HipOps(object):
     def __init__(self, device=None):
         if not torch.cuda.is_available():
@@ -111,6 +343,7 @@ class HipOps(object):
         self.range_flag = torch.zeros(1, dtype=torch.int32, device=self.device)
         # guard.run_guarded: passes re-run under the bf16x3 split because the fp16 pair met a value outside its range (0 in normal operation)
         self.fallbacks, self._fallback, self._guard_depth, self._range_scratch = 0, None, 0, None
+        self._captured_tables = []                       # tables of tensor lists that captured graphs read
 
     def cu_count(self):
         """Compute units of the device (the persistent kernels launch one workgroup per CU)."""
@@ -145,6 +378,64 @@ class HipOps(object):
 
     def _stream(self):
         return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def _index_device(self):
+        d = self.device
+        return d if d.index is not None else torch.device(d.type, torch.cuda.current_device())
+
+    def _on_device(self):
+        """A launch needs its device to be the current one."""
+        i = self.device.index
+        return contextlib.nullcontext() if i is None or i == torch.cuda.current_device() else torch.cuda.device(i)
+
+    # ---- lists of tensors: the end of a training step ------------------------------------------
+    def tensor_list(self, tensors, out=None, once=False):
+        """A handle of a list of gradients for grad_norm and clip_grads: dense float32 / float16 / bfloat16 tensors on this device, in any mixture, order of
+        axes and alignment, empty ones among them.  `out`: tensors of the same shapes, orders and types that take the clipped values (default: in place).
+
+        The handle stands for the memory that the tensors have now: their values are read at each call, but a gradient that is made anew (zero_grad with
+        set_to_none) needs a new handle.  Making one waits for the current stream; it may then be used on any stream, and in graphs, which have to be
+        captured after it was made.  once=True: a handle for the current stream alone, made without waiting, also while a graph is captured."""
+        return TensorList(self, tensors, out, once)
+
+    def grad_norm(self, tensors, norm_type=2.0, out=None):
+        """The norm of all elements of a tensor_list: 2 (summed in 64 bits, so finite gradients have a finite norm as far as float32 holds it) or inf.
+        NaN where an element is.  Returns a 0-d float32 on the device (`out`, if given)."""
+        norm_type = _norm_type(norm_type)
+        norm = self._norm_out(tensors, out)
+        if tensors.n:
+            with self._on_device():
+                a, stream, work = tensors.args(self, norm_type, norm)
+                _lib.check(self._launch(("grad_norm", tensors.n, tensors.count), lambda: self.lib.bfsr_grad_norm(C.byref(a), C.c_void_p(stream.cuda_stream))), "grad_norm")
+        return norm
+
+    def clip_grads(self, tensors, max_norm, norm_type=2.0):
+        """Multiplies a tensor_list by min(1, max_norm / (norm + 1e-6)), in place or into its `out`; returns the norm before (0-d float32, on the device).
+        An infinite norm makes finite gradients 0, a NaN makes all NaN, as the quotient does.  Products are rounded once, to the tensor's type."""
+        norm_type, max_norm = _norm_type(norm_type), _at_least_0(max_norm, "clip_grads.max_norm")
+        norm = self._norm_out(tensors, None)
+        if tensors.n:
+            with self._on_device():
+                a, stream, work = tensors.args(self, norm_type, norm)
+                _lib.check(self._launch(("clip_grads", tensors.n, tensors.count),
+                                        lambda: self.lib.bfsr_clip_grads(C.byref(a), max_norm, C.c_void_p(stream.cuda_stream))), "clip_grads")
+            torch.autograd.graph.increment_version(tensors.written)
+        return norm
+
+    def _norm_out(self, tensors, out):
+        if not isinstance(tensors, TensorList) or tensors.ops is not self:
+            raise TypeError("need a handle from this object's tensor_list()")
+        dev = self._index_device()
+        if out is not None:
+            _one_float(out, dev, "grad_norm.out")
+            return out if tensors.n else out.zero_()
+        return torch.empty((), dtype=torch.float32, device=dev) if tensors.n else torch.zeros((), dtype=torch.float32, device=dev)
+
+    def adam(self, params, grads, exp_avg, exp_avg_sq, step):
+        """A plan of Adam's update of `params` (float32 / float16 / bfloat16; gradients of any of these, moments float32, all in the parameter's shape and
+        order of axes).  grads=None: every run() brings its own, of the parameters' types, and the plan holds none.  step: the counts of steps taken, a 1-d float32 tensor or a list of tensors of one float32.  AdamPlan.run() makes a step.
+        Like a tensor_list, the plan stands for the memory that the tensors have now, and making it waits for the current stream."""
+        return AdamPlan(self, params, grads, exp_avg, exp_avg_sq, step)
 
     # ---- conv -----------------------------------------------------------------------------
     def _pack_raw(self, w, mtile):

@@ -1,0 +1,135 @@
+"""The end of a training step on the HIP kernels, for the modules that `linf/train.py` trains: gradient clipping by the global norm and Adam (the optimizer
+of LINF-LP/train.py:46-62).  Both take any list of dense float32 / float16 / bfloat16 parameters on one GPU in a few launches (ops.tensor_list, ops.adam),
+and neither waits for the device.
+
+`Adam` is a `torch.optim.Optimizer`: parameter groups, learning-rate schedulers and checkpoints work as with `torch.optim.Adam` / `AdamW`, whose
+state dicts it reads and whose state it writes (`step`, `exp_avg`, `exp_avg_sq`; moments are float32 whatever the parameter's type)."""
+import torch
+
+from .ops import HipOps, _order
+
+_shared = {}
+
+
+def _ops_of(t, ops=None):
+    """The ops object for the device of `t`: the given one, or one that calls without it share."""
+    if t.device.type != "cuda":
+        raise ValueError("bfsr_amd.optim: need parameters on a GPU, got one on %s" % t.device)
+    if ops is None:
+        ops = _shared.get(t.device)
+        if ops is None:
+            ops = _shared[t.device] = HipOps(t.device)
+    return ops
+
+
+def clip_grad_norm(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, ops=None):
+    """Scales the gradients of `parameters` (those that have one) in place so that their global norm (2 or inf) is at most `max_norm`; returns the norm before,
+    a 0-d float32 tensor on the device.  error_if_nonfinite: waits for the norm and raises if it is infinite or NaN (the gradients are then scaled already:
+    zero or NaN).  May be captured into a graph."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    ops = ops or _ops_of(grads[0])
+    norm = ops.clip_grads(ops.tensor_list(grads, once=True), max_norm, norm_type)
+    if error_if_nonfinite and not torch.isfinite(norm):
+        raise RuntimeError("bfsr_amd.optim.clip_grad_norm: the norm of the gradients is %r" % float(norm))
+    return norm
+
+
+class Adam(torch.optim.Optimizer):
+    """Adam, with L2 regularisation (`weight_decay`) or, with `decoupled_weight_decay`, AdamW's decay.
+
+    max_grad_norm     clip the gradients of all groups by their global norm, within the update: p.grad is left as it is
+    skip_nonfinite    a step whose gradients' norm is infinite or NaN changes nothing, step counts included
+    `grad_norm` holds the last step's norm (0-d, on the device) where one of the two is asked for.
+    A group's lr may be a tensor of one float32 on the device; a step captured into a graph then follows it.  Capture after one ordinary step."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled_weight_decay=False, max_grad_norm=None, skip_nonfinite=False,
+                 ops=None):
+        if not isinstance(lr, torch.Tensor) and not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError("Adam: lr %r, eps %r, weight_decay %r or betas %r out of range" % (lr, eps, weight_decay, betas))
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError("Adam: max_grad_norm %r is out of range" % (max_grad_norm,))
+        self.max_grad_norm, self.skip_nonfinite, self.grad_norm = max_grad_norm, skip_nonfinite, None
+        self._ops, self._plans = ops, {}
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, decoupled_weight_decay=decoupled_weight_decay))
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plans = {}
+        for name, value in (("_ops", None), ("max_grad_norm", None), ("skip_nonfinite", False), ("grad_norm", None)):
+            self.__dict__.setdefault(name, value)
+        for group in self.param_groups:
+            group.setdefault("decoupled_weight_decay", False)
+            if group.get("amsgrad") or group.get("maximize"):
+                raise ValueError("Adam: amsgrad and maximize are not supported")
+
+    def __getstate__(self):
+        return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm, skip_nonfinite=self.skip_nonfinite)
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # torch casts loaded moments to the parameter's type and leaves `step` where it was: take both from the dict as they are
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, [p for g in self.param_groups for p in g["params"]]):
+            loaded = state_dict["state"].get(i)
+            if loaded:
+                self.state[p] = {"step": torch.as_tensor(loaded["step"], dtype=torch.float32).detach().clone().reshape(()).to(p.device)}
+                for name in ("exp_avg", "exp_avg_sq"):
+                    self.state[p][name] = self._moment(p).copy_(loaded[name].detach())
+
+    @staticmethod
+    def _moment(p):
+        return torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format, requires_grad=False)
+
+    def _state_of(self, params):
+        new = [p for p in params if not self.state[p]]
+        if new:
+            for p, step in zip(new, torch.zeros(len(new), dtype=torch.float32, device=new[0].device).unbind()):
+                self.state[p] = {"step": step, "exp_avg": self._moment(p), "exp_avg_sq": self._moment(p)}
+        return [self.state[p] for p in params]
+
+    def _plan(self, at, ops, params, grads):
+        """The group's plan, if it still names the memory that parameters and state have, or a new one."""
+        state = self._state_of(params)
+        cols = [params] + [[s[k] for s in state] for k in ("exp_avg", "exp_avg_sq", "step")]
+        where = [t.data_ptr() for c in cols for t in c]
+        kinds = [g.dtype for g in grads]
+        held = self._plans.get(at)
+        if held is None or held[0] is not ops or held[1] != where or held[2] != kinds:
+            bring = all(k == p.dtype for k, p in zip(kinds, params))         # the plan holds no gradients, which zero_grad may want to free
+            held = self._plans[at] = (ops, where, kinds, ops.adam(cols[0], None if bring else grads, *cols[1:]))
+        return held[3]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work = []
+        for at, group in enumerate(self.param_groups):
+            params = [p for p in group["params"] if p.grad is not None]
+            if not params:
+                continue
+            grads = []
+            for p in params:
+                g = p.grad
+                if g.is_sparse:
+                    raise RuntimeError("Adam: sparse gradients are not supported")
+                grads.append(g if _order(g) == _order(p) else torch.empty_like(p, dtype=g.dtype).copy_(g))
+            ops = self._ops or _ops_of(params[0])
+            work.append((group, self._plan(at, ops, params, grads), grads, ops))
+        self.grad_norm = None
+        wants = self.max_grad_norm is not None or self.skip_nonfinite
+        norm = None
+        if wants and len(work) > 1:
+            ops = work[0][3]
+            norm = ops.grad_norm(ops.tensor_list([g for w in work for g in w[2]], once=True))
+        for group, plan, grads, ops in work:
+            got = plan.run(group["lr"], group["betas"], group["eps"], group["weight_decay"], group["decoupled_weight_decay"], self.max_grad_norm,
+                           grad_norm=norm, skip_nonfinite=self.skip_nonfinite, grads=grads)
+            self.grad_norm = got if norm is None else norm
+        return loss

@@ -592,6 +592,46 @@ int bfsr_ssim_sum_w(const float* a, long long a_bs, const float* b, long long b_
                     int ws, const double* window, double cov_norm, double* out, void* stream);
 int bfsr_to_uint8(const float* x, long long x_bs, unsigned char* y, int B, long long n, void* stream);
 
+/* ---- the end of a training step over a list of tensors (tensor_list.hip) ------------------------------------------------------------
+ * The optimizer's part of the latent module's training loop (LINF-LP/train.py:46-62, 118-163), and clipping before it.
+ * A list is n dense tensors, each flat memory of `sizes[k]` elements (any alignment that suits the element; sizes of 0 are taken).  Its table on the device is
+ * `rows` (BFSR_LIST_ROW bytes a row) and `chunks` (8 bytes for each started `chunk` elements of a row; `chunk` from bfsr_list_chunk), both the caller's,
+ * filled by bfsr_list_write and good for any number of later calls while the tensors stay where they are:
+ *   ncols 1: {tensor}, results go back to it; ncols 2: {tensor, where the result goes}, of one type;
+ *   ncols 5: {parameter, gradient, first moment, second moment, step count}: moments and the step count (one float a row) fp32.
+ * cols[c][k] and sizes / types are HOST arrays, read before the call returns (they travel as kernel arguments: the call does not wait, and may be captured).
+ * types[k] = type of the tensor | type of the gradient << 4 (ncols 5).  No two tensors that a call writes may overlap.
+ * bfsr_pointer_write: the same for a bare array of n pointers on the device (BfsrListArgs.other).
+ *   bfsr_grad_norm : norm = sqrt(sum g^2), summed in 64 bits in an order fixed by the list (max: the largest |g|); NaN where an element is one.
+ *   bfsr_clip_grads: out = g * min(1, max_norm / (norm + 1e-6)); `norm` gets the norm before it.
+ *   bfsr_adam_step : t += 1; g *= share (max_norm >= 0); p *= 1 - lr wd (decoupled) or g += wd p; m = b1 m + (1 - b1) g; v = b2 v + (1 - b2) g^2;
+ *                    p -= lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps), in 32 bits, factors in 64, p rounded once to its type. */
+#define BFSR_LIST_ROW 64
+enum { BFSR_LIST_F32 = 0, BFSR_LIST_F16 = 1, BFSR_LIST_BF16 = 2 };
+typedef struct BfsrListArgs {
+    const void* rows; const void* chunks;    /* the table */
+    int n, count, chunk;                     /* rows, chunks, elements a chunk */
+    int max;                                 /* the norm: 0 Euclidean, 1 the largest magnitude */
+    const void* other;                       /* bfsr_adam_step: NULL, or the gradients' n pointers in place of the table's (same sizes and types) */
+    void* work;                              /* scratch of this call alone, bfsr_list_work(n) bytes, 16-byte aligned */
+    float* norm;                             /* where the norm goes (bfsr_adam_step: only with max_norm >= 0 or skip_nonfinite) */
+} BfsrListArgs;
+typedef struct BfsrAdamArgs {
+    double lr; const float* lr_at;           /* the rate, or (not NULL) where it stands on the device */
+    double beta1, beta2, weight_decay; float eps;
+    int decoupled;                           /* decay of the parameters themselves in place of an added gradient */
+    float max_norm;                          /* < 0: no clipping */
+    const float* given_norm;                 /* NULL, or the norm to clip by in place of this list's own */
+    int skip_nonfinite;                      /* leave everything as it is, step counts too, where the norm is not finite */
+} BfsrAdamArgs;
+int bfsr_list_chunk(long long total);                      /* elements a chunk for a list of `total` elements */
+long long bfsr_list_work(int n);                           /* bytes of scratch */
+int bfsr_list_write(const void* const* const* cols, int ncols, const long long* sizes, const int* types, int n, int chunk, void* rows, void* chunks, void* stream);
+int bfsr_pointer_write(const void* const* from, int n, void* to, void* stream);
+int bfsr_grad_norm(const BfsrListArgs* a, void* stream);
+int bfsr_clip_grads(const BfsrListArgs* a, float max_norm, void* stream);
+int bfsr_adam_step(const BfsrListArgs* a, const BfsrAdamArgs* h, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
