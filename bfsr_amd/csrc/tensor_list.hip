@@ -16,7 +16,8 @@
 namespace {
 
 constexpr int T = 256;                        // threads of a workgroup
-constexpr int STEP = T * 4;                   // elements that a workgroup takes at a time, four for each lane
+constexpr int WAVES = T / 64;
+constexpr int CHUNK = 2048;                   // elements of a chunk: what one wave takes at a time
 constexpr int MAX_PARTS = 1024;               // partial results of a norm, one for each of its workgroups
 
 struct Row { const void* p[4]; float* step; long long n; int type, type_g; long long pad; };      // BFSR_LIST_ROW bytes
@@ -25,6 +26,7 @@ static_assert(sizeof(Row) == BFSR_LIST_ROW, "the row's size is part of the inter
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short h4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned short h8u __attribute__((ext_vector_type(8), aligned(2)));
 #define GLOBAL __attribute__((address_space(1)))          // the rows' pointers are of device memory, which the compiler cannot know: without it every access is a flat one
 
 __device__ __forceinline__ float from_half(unsigned short h) { return __half2float(__ushort_as_half(h)); }
@@ -36,38 +38,56 @@ __device__ __forceinline__ unsigned short to_bf16(float f)               // roun
     return f != f ? (unsigned short)((u >> 16) | 0x40) : (unsigned short)((u + 0x7fff + ((u >> 16) & 1)) >> 16);
 }
 
-// Element i .. i+3 of a tensor of `type` as floats; those from n on are 0.
-__device__ __forceinline__ f4 load4(const void* p, int type, long long i, long long n)
+// The elements of a type, N to a load of 16 bytes.
+template <int TYPE> struct Vec;
+template <> struct Vec<BFSR_LIST_F32> { typedef f4u type; typedef float one; static constexpr int N = 4; __device__ static float wide(float f) { return f; } };
+template <> struct Vec<BFSR_LIST_F16> { typedef h8u type; typedef unsigned short one; static constexpr int N = 8; __device__ static float wide(unsigned short h) { return from_half(h); } };
+template <> struct Vec<BFSR_LIST_BF16> { typedef h8u type; typedef unsigned short one; static constexpr int N = 8; __device__ static float wide(unsigned short h) { return from_bf16(h); } };
+
+// Four elements of a tensor of `type` from element i on; those from `count` on are 0 and are not touched.
+struct Four { f4u f; h4u h; };
+
+template <bool FULL>
+__device__ __forceinline__ Four load4(const void* p, int type, int i, int count)
 {
-    f4 r = {0.f, 0.f, 0.f, 0.f};
+    Four r = {{0.f, 0.f, 0.f, 0.f}, {0, 0, 0, 0}};
     if (type == BFSR_LIST_F32) {
         const GLOBAL float* q = (const GLOBAL float*)p + i;
-        if (i + 4 <= n) return *(const GLOBAL f4u*)q;
-        for (int k = 0; k < 3; ++k) if (i + k < n) r[k] = q[k];
-        return r;
+        if (FULL || i + 4 <= count) r.f = *(const GLOBAL f4u*)q;
+        else for (int k = 0; k < 3; ++k) if (i + k < count) r.f[k] = q[k];
+    } else {
+        const GLOBAL unsigned short* q = (const GLOBAL unsigned short*)p + i;
+        if (FULL || i + 4 <= count) r.h = *(const GLOBAL h4u*)q;
+        else for (int k = 0; k < 3; ++k) if (i + k < count) r.h[k] = q[k];
     }
-    const GLOBAL unsigned short* q = (const GLOBAL unsigned short*)p + i;
-    h4u h = {0, 0, 0, 0};
-    if (i + 4 <= n) h = *(const GLOBAL h4u*)q;
-    else for (int k = 0; k < 3; ++k) if (i + k < n) h[k] = q[k];
-    for (int k = 0; k < 4; ++k) r[k] = type == BFSR_LIST_F16 ? from_half(h[k]) : from_bf16(h[k]);
     return r;
 }
 
-__device__ __forceinline__ void store4(void* p, int type, long long i, long long n, f4 v)
+__device__ __forceinline__ f4 floats(Four a, int type)
+{
+    if (type == BFSR_LIST_F32) return a.f;
+    f4 r;
+    for (int k = 0; k < 4; ++k) r[k] = type == BFSR_LIST_F16 ? from_half(a.h[k]) : from_bf16(a.h[k]);
+    return r;
+}
+
+template <bool FULL>
+__device__ __forceinline__ void store4(void* p, int type, int i, int count, f4 v)
 {
     if (type == BFSR_LIST_F32) {
         GLOBAL float* q = (GLOBAL float*)p + i;
-        if (i + 4 <= n) *(GLOBAL f4u*)q = v;
-        else for (int k = 0; k < 3; ++k) if (i + k < n) q[k] = v[k];
+        if (FULL || i + 4 <= count) *(GLOBAL f4u*)q = v;
+        else for (int k = 0; k < 3; ++k) if (i + k < count) q[k] = v[k];
         return;
     }
     GLOBAL unsigned short* q = (GLOBAL unsigned short*)p + i;
     h4u h;
     for (int k = 0; k < 4; ++k) h[k] = type == BFSR_LIST_F16 ? to_half(v[k]) : to_bf16(v[k]);
-    if (i + 4 <= n) *(GLOBAL h4u*)q = h;
-    else for (int k = 0; k < 3; ++k) if (i + k < n) q[k] = h[k];
+    if (FULL || i + 4 <= count) *(GLOBAL h4u*)q = h;
+    else for (int k = 0; k < 3; ++k) if (i + k < count) q[k] = h[k];
 }
+
+__device__ __forceinline__ void* at_element(const void* p, int type, long long i) { return (char*)p + i * (type == BFSR_LIST_F32 ? 4 : 2); }
 
 // The larger magnitude, where a NaN on either side wins (fmax would drop it).
 __device__ __forceinline__ double worse(double a, double b) { return (b > a || b != b) ? b : a; }
@@ -89,21 +109,55 @@ __device__ __forceinline__ double block_join(double v)
 }
 
 // Squares are formed and added in 64 bits: fp32's largest value squared overflows 32 bits, its smallest vanish, and a norm of finite gradients has to be finite.
+// Bound by memory: two instructions an element for the conversion and the multiply-add.  Each wave takes chunks of its own, 16 bytes a load and a chunk's loads all under way
+// at once; loads of 8 bytes one at a time kept 8 KB in flight per CU and reached 2.7 TB/s.
+template <bool MAX>
+__device__ __forceinline__ double take(double acc, float g) { return MAX ? join<true>(acc, (double)fabsf(g)) : fma((double)g, (double)g, acc); }
+
+template <bool MAX, int TYPE, bool FULL>
+__device__ __forceinline__ double take_chunk(double acc, const void* p, long long begin, int count)
+{
+    typedef typename Vec<TYPE>::type V;
+    constexpr int N = Vec<TYPE>::N, U = CHUNK / (64 * N);
+    const GLOBAL typename Vec<TYPE>::one* q = (const GLOBAL typename Vec<TYPE>::one*)p + begin;
+    const int lane = threadIdx.x & 63;
+    V g[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i = (u * 64 + lane) * N;
+        if (FULL || i + N <= count) g[u] = *(const GLOBAL V*)(q + i);
+        else {
+            g[u] = V{};
+            for (int k = 0; k < N - 1; ++k) if (i + k < count) g[u][k] = q[i + k];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        for (int k = 0; k < N; ++k) acc = take<MAX>(acc, Vec<TYPE>::wide(g[u][k]));
+    return acc;
+}
+
+template <bool MAX, int TYPE>
+__device__ __forceinline__ double take_chunk(double acc, const void* p, long long begin, int count)
+{
+    return count == CHUNK ? take_chunk<MAX, TYPE, true>(acc, p, begin, count) : take_chunk<MAX, TYPE, false>(acc, p, begin, count);
+}
+
 template <bool MAX>
 __global__ __launch_bounds__(T) void norm_parts_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other,
-                                                       int col, int count, int chunk, double* __restrict__ parts)
+                                                       int col, int count, double* __restrict__ parts)
 {
     double acc = 0.0;
-    for (int c = blockIdx.x; c < count; c += gridDim.x) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int c = blockIdx.x * WAVES + wave; c < count; c += gridDim.x * WAVES) {
         const int2 at = chunks[c];
         const Row& r = rows[at.x];
         const void* p = other ? other[at.x] : r.p[col];
         const int type = col ? r.type_g : r.type;
-        const long long n = r.n, begin = (long long)at.y * chunk, end = begin + chunk < n ? begin + chunk : n;
-        for (long long i = begin + threadIdx.x * 4; i < end; i += STEP) {
-            const f4 g = load4(p, type, i, end);
-            for (int k = 0; k < 4; ++k) acc = MAX ? join<true>(acc, (double)fabsf(g[k])) : fma((double)g[k], (double)g[k], acc);
-        }
+        const long long begin = (long long)at.y * CHUNK, left = r.n - begin;
+        const int here = left < CHUNK ? (int)left : CHUNK;
+        acc = type == BFSR_LIST_F32 ? take_chunk<MAX, BFSR_LIST_F32>(acc, p, begin, here) : type == BFSR_LIST_F16 ? take_chunk<MAX, BFSR_LIST_F16>(acc, p, begin, here)
+                                                                                                                 : take_chunk<MAX, BFSR_LIST_BF16>(acc, p, begin, here);
     }
     acc = block_join<MAX>(acc);
     if (threadIdx.x == 0) parts[blockIdx.x] = acc;
@@ -140,18 +194,31 @@ __device__ double finish(const Final& f)
 
 __global__ __launch_bounds__(T) void norm_finish_kernel(Final f) { finish(f); }
 
-__global__ __launch_bounds__(T) void clip_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, int chunk, const float* __restrict__ share)
+template <bool FULL>
+__device__ __forceinline__ void clip_chunk(const void* from, void* to, int type, int count, float s)
 {
-    const int2 at = chunks[blockIdx.x];
+    const int lane = threadIdx.x & 63;
+    constexpr int U = CHUNK / 256;
+    Four g[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) g[u] = load4<FULL>(from, type, (u * 64 + lane) * 4, count);
+#pragma unroll
+    for (int u = 0; u < U; ++u) store4<FULL>(to, type, (u * 64 + lane) * 4, count, floats(g[u], type) * s);
+}
+
+__global__ __launch_bounds__(T) void clip_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, int count, const float* __restrict__ share)
+{
+    const int c = blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (c >= count) return;
+    const int2 at = chunks[c];
     const Row& r = rows[at.x];
     const float s = *share;
     if (s == 1.f && r.p[0] == r.p[1]) return;                  // in place, and nothing to change
-    const long long begin = (long long)at.y * chunk, end = begin + chunk < r.n ? begin + chunk : r.n;
-    for (long long i = begin + threadIdx.x * 4; i < end; i += STEP) {
-        f4 g = load4(r.p[0], r.type, i, end);
-        for (int k = 0; k < 4; ++k) g[k] *= s;
-        store4((void*)r.p[1], r.type, i, end, g);
-    }
+    const long long begin = (long long)at.y * CHUNK, left = r.n - begin;
+    const void* from = at_element(r.p[0], r.type, begin);
+    void* to = at_element(r.p[1], r.type, begin);
+    if (left >= CHUNK) clip_chunk<true>(from, to, r.type, CHUNK, s);
+    else clip_chunk<false>(from, to, r.type, (int)left, s);
 }
 
 struct Hyper { double lr, beta1, beta2, weight_decay; float eps; int decoupled, skip; const float* lr_at; };
@@ -173,33 +240,60 @@ __global__ __launch_bounds__(T) void adam_begin_kernel(const Row* __restrict__ r
     }
 }
 
-__global__ __launch_bounds__(T) void adam_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other, int chunk,
+struct Rule { float share, b1, c1, b2, c2, wd, eps; bool add, keep; Factors f; };
+
+template <bool FULL>
+__device__ __forceinline__ void adam_chunk(void* pp, const void* gp, float* mp, float* vp, int type, int type_g, int count, const Rule& w)
+{
+    const int lane = threadIdx.x & 63;
+    constexpr int U = 2;
+    for (int j = 0; j < CHUNK && (FULL || j < count); j += U * 256) {
+        Four p[U], g[U], m[U], v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = j + (u * 64 + lane) * 4;
+            p[u] = load4<FULL>(pp, type, i, count);
+            g[u] = load4<FULL>(gp, type_g, i, count);
+            m[u] = load4<FULL>(mp, BFSR_LIST_F32, i, count);
+            v[u] = load4<FULL>(vp, BFSR_LIST_F32, i, count);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = j + (u * 64 + lane) * 4;
+            f4 x = floats(p[u], type), y = floats(g[u], type_g), m1, v1;
+            for (int k = 0; k < 4; ++k) {
+                float d = y[k] * w.share;
+                if (w.add) d = fmaf(w.wd, x[k], d);
+                if (w.keep) x[k] *= w.f.keep;
+                m1[k] = fmaf(w.b1, m[u].f[k], w.c1 * d);
+                v1[k] = fmaf(w.b2, v[u].f[k], w.c2 * d * d);
+                x[k] -= w.f.size * (m1[k] / fmaf(sqrtf(v1[k]), w.f.root, w.eps));
+            }
+            store4<FULL>(pp, type, i, count, x);
+            store4<FULL>(mp, BFSR_LIST_F32, i, count, m1);
+            store4<FULL>(vp, BFSR_LIST_F32, i, count, v1);
+        }
+    }
+}
+
+__global__ __launch_bounds__(T) void adam_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other, int count,
                                                  Hyper h, const Factors* __restrict__ factors, const float* __restrict__ share)
 {
-    const int2 at = chunks[blockIdx.x];
+    const int c = blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (c >= count) return;
+    const int2 at = chunks[c];
     const Row& r = rows[at.x];
     const Factors f = factors[at.x];
     if (f.go == 0.f) return;
-    const float s = *share, b1 = (float)h.beta1, c1 = (float)(1.0 - h.beta1), b2 = (float)h.beta2, c2 = (float)(1.0 - h.beta2), wd = (float)h.weight_decay;
-    const bool add = wd != 0.f && !h.decoupled, keep = wd != 0.f && h.decoupled;
-    const void* gp = other ? other[at.x] : r.p[1];
-    float* mp = (float*)r.p[2];
-    float* vp = (float*)r.p[3];
-    const long long begin = (long long)at.y * chunk, end = begin + chunk < r.n ? begin + chunk : r.n;
-    for (long long i = begin + threadIdx.x * 4; i < end; i += STEP) {
-        f4 p = load4(r.p[0], r.type, i, end), g = load4(gp, r.type_g, i, end), m = load4(mp, BFSR_LIST_F32, i, end), v = load4(vp, BFSR_LIST_F32, i, end);
-        for (int k = 0; k < 4; ++k) {
-            float x = g[k] * s;
-            if (add) x = fmaf(wd, p[k], x);
-            if (keep) p[k] *= f.keep;
-            m[k] = fmaf(b1, m[k], c1 * x);
-            v[k] = fmaf(b2, v[k], c2 * x * x);
-            p[k] -= f.size * (m[k] / fmaf(sqrtf(v[k]), f.root, h.eps));
-        }
-        store4((void*)r.p[0], r.type, i, end, p);
-        store4(mp, BFSR_LIST_F32, i, end, m);
-        store4(vp, BFSR_LIST_F32, i, end, v);
-    }
+    const float wd = (float)h.weight_decay;
+    const Rule w = {*share, (float)h.beta1, (float)(1.0 - h.beta1), (float)h.beta2, (float)(1.0 - h.beta2), wd, h.eps, wd != 0.f && !h.decoupled, wd != 0.f && h.decoupled, f};
+    const long long begin = (long long)at.y * CHUNK, left = r.n - begin;
+    void* p = at_element(r.p[0], r.type, begin);
+    const void* g = at_element(other ? other[at.x] : r.p[1], r.type_g, begin);
+    float* m = (float*)r.p[2] + begin;
+    float* v = (float*)r.p[3] + begin;
+    if (left >= CHUNK) adam_chunk<true>(p, g, m, v, r.type, r.type_g, CHUNK, w);
+    else adam_chunk<false>(p, g, m, v, r.type, r.type_g, (int)left, w);
 }
 
 // ---- the table: rows and chunks travel to the device as kernel arguments.  No host buffer has to outlive the call, nothing waits for the stream, and a
@@ -254,27 +348,28 @@ __global__ __launch_bounds__(512) void pointer_write_kernel(Pointers all, int n,
     if ((int)threadIdx.x < n) to[threadIdx.x] = all.p[threadIdx.x];
 }
 
-bool good(const BfsrListArgs& a) { return a.rows && a.chunks && a.n > 0 && a.count >= 0 && a.count < (1 << 24) && a.chunk > 0 && a.chunk % STEP == 0; }
+bool good(const BfsrListArgs& a) { return a.rows && a.chunks && a.n > 0 && a.count >= 0 && a.count < (1 << 24) && a.chunk == CHUNK; }
 
-int parts_of(int count) { return count < MAX_PARTS ? count : MAX_PARTS; }
+int blocks_of(int count) { return (count + WAVES - 1) / WAVES; }
+int parts_of(int count) { return blocks_of(count) < MAX_PARTS ? blocks_of(count) : MAX_PARTS; }
 
 int launch_parts(const BfsrListArgs& a, int col, double* parts, hipStream_t st)
 {
     if (!a.count) return 0;
     const auto k = a.max ? norm_parts_kernel<true> : norm_parts_kernel<false>;
-    k<<<parts_of(a.count), T, 0, st>>>((const Row*)a.rows, (const int2*)a.chunks, (const void* const*)a.other, col, a.count, a.chunk, parts);
+    k<<<parts_of(a.count), T, 0, st>>>((const Row*)a.rows, (const int2*)a.chunks, (const void* const*)a.other, col, a.count, parts);
     return (int)hipGetLastError();
 }
 
 }  // namespace
 
-extern "C" int bfsr_list_chunk(long long total) { return total < 0 ? -1 : 4 * STEP; }
+extern "C" int bfsr_list_chunk(long long total) { return total < 0 ? -1 : CHUNK; }
 
 extern "C" long long bfsr_list_work(int n) { return n < 0 ? -1 : (long long)MAX_PARTS * 8 + 16 + (long long)n * (long long)sizeof(Factors); }
 
 extern "C" int bfsr_list_write(const void* const* const* cols, int ncols, const long long* sizes, const int* types, int n, int chunk, void* rows, void* chunks, void* stream)
 {
-    if (!cols || !sizes || !types || n <= 0 || chunk <= 0 || chunk % STEP || !rows || !chunks) return -1;
+    if (!cols || !sizes || !types || n <= 0 || chunk != CHUNK || !rows || !chunks) return -1;
     if (ncols != 1 && ncols != 2 && ncols != 5) return -1;
     long long count = 0;
     for (int k = 0; k < n; ++k) {
@@ -327,7 +422,7 @@ extern "C" int bfsr_clip_grads(const BfsrListArgs* a, float max_norm, void* stre
     const int err = launch_parts(*a, 0, parts, st);
     if (err) return err;
     norm_finish_kernel<<<1, T, 0, st>>>(Final{parts, parts_of(a->count), a->max, nullptr, a->norm, max_norm, share});
-    if (a->count) clip_kernel<<<a->count, T, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, a->chunk, share);
+    if (a->count) clip_kernel<<<blocks_of(a->count), T, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, a->count, share);
     return (int)hipGetLastError();
 }
 
@@ -349,6 +444,6 @@ extern "C" int bfsr_adam_step(const BfsrListArgs* a, const BfsrAdamArgs* h, void
     const Hyper hy = {h->lr, h->beta1, h->beta2, h->weight_decay, h->eps, h->decoupled, h->skip_nonfinite, h->lr_at};
     adam_begin_kernel<<<1, T, 0, st>>>((const Row*)a->rows, a->n, Final{parts, own ? parts_of(a->count) : 0, a->max, norm ? h->given_norm : nullptr, norm ? a->norm : nullptr,
                                        h->max_norm >= 0.f ? h->max_norm : -1.f, share}, hy, factors);
-    if (a->count) adam_kernel<<<a->count, T, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, (const void* const*)a->other, a->chunk, hy, factors, share);
+    if (a->count) adam_kernel<<<blocks_of(a->count), T, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, (const void* const*)a->other, a->count, hy, factors, share);
     return (int)hipGetLastError();
 }
