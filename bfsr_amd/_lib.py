@@ -178,7 +178,7 @@ class BfsrListArgs(C.Structure):
     _fields_ = [
         ("rows", C.c_void_p), ("chunks", C.c_void_p),
         ("n", C.c_int), ("count", C.c_int), ("chunk", C.c_int), ("max", C.c_int),
-        ("other", C.c_void_p), ("work", C.c_void_p), ("norm", C.c_void_p),
+        ("other", C.c_void_p), ("bytes", C.c_longlong), ("work", C.c_void_p), ("norm", C.c_void_p),
     ]
 
 

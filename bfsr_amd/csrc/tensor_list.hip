@@ -15,16 +15,21 @@
 
 namespace {
 
-constexpr int T = 256;                        // threads of a workgroup
-constexpr int WAVES = T / 64;
-constexpr int CHUNK = 2048;                   // elements of a chunk: what one wave takes at a time
-constexpr int MAX_PARTS = 1024;               // partial results of a norm, one for each of its workgroups
+constexpr int T = 256;                        // threads of a workgroup that updates
+constexpr int TN = 1024;                      // threads of one that sums
+constexpr int CHUNK = 2048;                   // elements of a chunk
+constexpr int PARTS = 256;                    // partial results of a norm at most, one for each of its workgroups: one a CU, and four a lane for the wave that joins them
+constexpr int ALONE = 16;                     // chunks up to which one workgroup sums a list by itself
+constexpr long long CACHE = 128ll << 20;      // bytes of tensors up to which a call counts on finding, and leaves, them in the 256 MB cache that the card shares
 
 struct Row { const void* p[4]; float* step; long long n; int type, type_g; long long pad; };      // BFSR_LIST_ROW bytes
 static_assert(sizeof(Row) == BFSR_LIST_ROW, "the row's size is part of the interface");
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned short h2 __attribute__((ext_vector_type(2)));
+typedef unsigned short h4 __attribute__((ext_vector_type(4)));
+typedef unsigned short h8 __attribute__((ext_vector_type(8)));
 typedef unsigned short h4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned short h8u __attribute__((ext_vector_type(8), aligned(2)));
 #define GLOBAL __attribute__((address_space(1)))          // the rows' pointers are of device memory, which the compiler cannot know: without it every access is a flat one
@@ -38,28 +43,33 @@ __device__ __forceinline__ unsigned short to_bf16(float f)               // roun
     return f != f ? (unsigned short)((u >> 16) | 0x40) : (unsigned short)((u + 0x7fff + ((u >> 16) & 1)) >> 16);
 }
 
+// STREAM: past the shared cache, for lists that it cannot hold anyway.  Read that way 614 MB came in at 6.4 TB/s, the usual way at 4.1; what follows on a list
+// that fits (an update after a norm, the next step) found it in the cache the usual way and lost 10 to 20 % the other.
+// (written out for each type: a template's argument would lose the alignment that the typedefs carry)
+#define ACCESS(V, ONE, LOAD, STORE) \
+    template <bool STREAM> __device__ __forceinline__ V LOAD(const GLOBAL ONE* p) \
+    { if constexpr (STREAM) return __builtin_nontemporal_load((const GLOBAL V##u*)p); else return *(const GLOBAL V##u*)p; } \
+    template <bool STREAM> __device__ __forceinline__ void STORE(GLOBAL ONE* p, V v) \
+    { if constexpr (STREAM) __builtin_nontemporal_store((V##u)v, (GLOBAL V##u*)p); else *(GLOBAL V##u*)p = v; }
+ACCESS(f4, float, load16, store16)
+ACCESS(h8, unsigned short, load16, store16)
+ACCESS(h4, unsigned short, load8, store8)
+
 // The elements of a type, N to a load of 16 bytes.
 template <int TYPE> struct Vec;
-template <> struct Vec<BFSR_LIST_F32> { typedef f4u type; typedef float one; static constexpr int N = 4; __device__ static float wide(float f) { return f; } };
-template <> struct Vec<BFSR_LIST_F16> { typedef h8u type; typedef unsigned short one; static constexpr int N = 8; __device__ static float wide(unsigned short h) { return from_half(h); } };
-template <> struct Vec<BFSR_LIST_BF16> { typedef h8u type; typedef unsigned short one; static constexpr int N = 8; __device__ static float wide(unsigned short h) { return from_bf16(h); } };
+template <> struct Vec<BFSR_LIST_F32> { typedef f4 type; typedef float one; static constexpr int N = 4; __device__ static float wide(float f) { return f; } __device__ static float narrow(float f) { return f; } };
+template <> struct Vec<BFSR_LIST_F16> { typedef h8 type; typedef unsigned short one; static constexpr int N = 8; __device__ static float wide(unsigned short h) { return from_half(h); } __device__ static unsigned short narrow(float f) { return to_half(f); } };
+template <> struct Vec<BFSR_LIST_BF16> { typedef h8 type; typedef unsigned short one; static constexpr int N = 8; __device__ static float wide(unsigned short h) { return from_bf16(h); } __device__ static unsigned short narrow(float f) { return to_bf16(f); } };
 
-// Four elements of a tensor of `type` from element i on; those from `count` on are 0 and are not touched.
-struct Four { f4u f; h4u h; };
+// Four elements of a tensor of `type` from element i on.
+struct Four { f4 f; h4 h; };
 
-template <bool FULL>
-__device__ __forceinline__ Four load4(const void* p, int type, int i, int count)
+template <bool STREAM>
+__device__ __forceinline__ Four load4(const void* p, int type, int i)
 {
-    Four r = {{0.f, 0.f, 0.f, 0.f}, {0, 0, 0, 0}};
-    if (type == BFSR_LIST_F32) {
-        const GLOBAL float* q = (const GLOBAL float*)p + i;
-        if (FULL || i + 4 <= count) r.f = *(const GLOBAL f4u*)q;
-        else for (int k = 0; k < 3; ++k) if (i + k < count) r.f[k] = q[k];
-    } else {
-        const GLOBAL unsigned short* q = (const GLOBAL unsigned short*)p + i;
-        if (FULL || i + 4 <= count) r.h = *(const GLOBAL h4u*)q;
-        else for (int k = 0; k < 3; ++k) if (i + k < count) r.h[k] = q[k];
-    }
+    Four r;
+    if (type == BFSR_LIST_F32) r.f = load16<STREAM>((const GLOBAL float*)p + i);
+    else r.h = load8<STREAM>((const GLOBAL unsigned short*)p + i);
     return r;
 }
 
@@ -71,51 +81,83 @@ __device__ __forceinline__ f4 floats(Four a, int type)
     return r;
 }
 
-template <bool FULL>
-__device__ __forceinline__ void store4(void* p, int type, int i, int count, f4 v)
+template <bool STREAM>
+__device__ __forceinline__ void store4(void* p, int type, int i, f4 v)
 {
-    if (type == BFSR_LIST_F32) {
-        GLOBAL float* q = (GLOBAL float*)p + i;
-        if (FULL || i + 4 <= count) *(GLOBAL f4u*)q = v;
-        else for (int k = 0; k < 3; ++k) if (i + k < count) q[k] = v[k];
-        return;
-    }
-    GLOBAL unsigned short* q = (GLOBAL unsigned short*)p + i;
-    h4u h;
+    if (type == BFSR_LIST_F32) return store16<STREAM>((GLOBAL float*)p + i, v);
+    h4 h;
     for (int k = 0; k < 4; ++k) h[k] = type == BFSR_LIST_F16 ? to_half(v[k]) : to_bf16(v[k]);
-    if (FULL || i + 4 <= count) *(GLOBAL h4u*)q = h;
-    else for (int k = 0; k < 3; ++k) if (i + k < count) q[k] = h[k];
+    store8<STREAM>((GLOBAL unsigned short*)p + i, h);
 }
+
+__device__ __forceinline__ float load1(const void* p, int type, int i)
+{
+    if (type == BFSR_LIST_F32) return ((const GLOBAL float*)p)[i];
+    const unsigned short h = ((const GLOBAL unsigned short*)p)[i];
+    return type == BFSR_LIST_F16 ? from_half(h) : from_bf16(h);
+}
+
+__device__ __forceinline__ void store1(void* p, int type, int i, float v)
+{
+    if (type == BFSR_LIST_F32) ((GLOBAL float*)p)[i] = v;
+    else ((GLOBAL unsigned short*)p)[i] = type == BFSR_LIST_F16 ? to_half(v) : to_bf16(v);
+}
+
+// Elements of the chunk that begins at element `begin`.
+__device__ __forceinline__ int left_in(const Row& r, long long begin) { return r.n - begin < CHUNK ? (int)(r.n - begin) : CHUNK; }
 
 __device__ __forceinline__ void* at_element(const void* p, int type, long long i) { return (char*)p + i * (type == BFSR_LIST_F32 ? 4 : 2); }
 
-// The larger magnitude, where a NaN on either side wins (fmax would drop it).
-__device__ __forceinline__ double worse(double a, double b) { return (b > a || b != b) ? b : a; }
-
-template <bool MAX>
-__device__ __forceinline__ double join(double a, double b) { return MAX ? (a != a ? a : worse(a, b)) : a + b; }
-
-// The join of one value of each thread, in an order that depends on nothing but the number of threads; thread 0 has it.
-template <bool MAX>
-__device__ __forceinline__ double block_join(double v)
-{
-    __shared__ double part[T / 64];
+// The sum of squares, or the largest magnitude, of what a thread has seen.
+// Squares are formed and added in 64 bits: fp32's largest value squared overflows 32 bits, its smallest vanish, and a norm of finite gradients has to be finite.
+// Magnitudes are compared as whole numbers: without the sign, larger bits are a larger number, infinity is above them all and NaN above that, so a NaN stays (fmax
+// would drop it), at one instruction an element; compared in 64 bits as the sums are, 38 M elements took 20 us and not the 12 that memory needs.
+template <bool MAX> struct Acc;
+template <> struct Acc<false> {
+    double a = 0.0;
+    __device__ __forceinline__ void join(double b) { a += b; }
+    template <int TYPE> __device__ __forceinline__ void take(typename Vec<TYPE>::type g)
+    {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = join<MAX>(v, __shfl_down(v, o, 64));
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
-    for (int k = 1; k < T / 64; ++k) v = join<MAX>(v, part[k]);
-    return v;
+        for (int k = 0; k < Vec<TYPE>::N; ++k) { const double d = (double)Vec<TYPE>::wide(g[k]); a = fma(d, d, a); }
+    }
+    __device__ __forceinline__ double part() const { return a; }
+    __device__ static double whole(double sum) { return sqrt(sum); }
+};
+template <> struct Acc<true> {
+    unsigned a = 0;
+    __device__ __forceinline__ void join(double b) { const unsigned u = __float_as_uint((float)b); a = max(a, u); }
+    template <int TYPE> __device__ __forceinline__ void take(typename Vec<TYPE>::type g)
+    {
+        if constexpr (TYPE == BFSR_LIST_F32) {
+            const auto bits = [](float f) { return __float_as_uint(f) & 0x7fffffffu; };
+            a = max(max(a, max(bits(g.x), bits(g.y))), max(bits(g.z), bits(g.w)));
+        } else {
+            g &= (unsigned short)0x7fff;
+            const h4 h = __builtin_elementwise_max(g.lo, g.hi);
+            const h2 l = __builtin_elementwise_max(h.lo, h.hi);
+            a = max(a, __float_as_uint(Vec<TYPE>::wide(l.x > l.y ? l.x : l.y)));
+        }
+    }
+    __device__ __forceinline__ double part() const { return (double)__uint_as_float(a); }
+    __device__ static double whole(double most) { return most; }
+};
+
+// The join over a wave, in an order that depends on nothing; every lane has it.
+template <bool MAX>
+__device__ __forceinline__ double wave_join(double v)
+{
+    Acc<MAX> acc;
+    acc.join(v);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) acc.join(__shfl_xor(acc.part(), o, 64));
+    return acc.part();
 }
 
-// Squares are formed and added in 64 bits: fp32's largest value squared overflows 32 bits, its smallest vanish, and a norm of finite gradients has to be finite.
-// Bound by memory: two instructions an element for the conversion and the multiply-add.  Each wave takes chunks of its own, 16 bytes a load and a chunk's loads all under way
-// at once; loads of 8 bytes one at a time kept 8 KB in flight per CU and reached 2.7 TB/s.
-template <bool MAX>
-__device__ __forceinline__ double take(double acc, float g) { return MAX ? join<true>(acc, (double)fabsf(g)) : fma((double)g, (double)g, acc); }
-
-template <bool MAX, int TYPE, bool FULL>
-__device__ __forceinline__ double take_chunk(double acc, const void* p, long long begin, int count)
+// One chunk for one wave, 16 bytes a load and all of them under way at once.  Bound by memory; with loads of 8 bytes one at a time 8 KB were in flight per CU
+// and 2.7 TB/s came in.
+template <bool MAX, bool STREAM, int TYPE>
+__device__ __forceinline__ void take_chunk(Acc<MAX>& acc, const void* p, long long begin, int count)
 {
     typedef typename Vec<TYPE>::type V;
     constexpr int N = Vec<TYPE>::N, U = CHUNK / (64 * N);
@@ -125,175 +167,259 @@ __device__ __forceinline__ double take_chunk(double acc, const void* p, long lon
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int i = (u * 64 + lane) * N;
-        if (FULL || i + N <= count) g[u] = *(const GLOBAL V*)(q + i);
-        else {
-            g[u] = V{};
-            for (int k = 0; k < N - 1; ++k) if (i + k < count) g[u][k] = q[i + k];
-        }
+        g[u] = V{};
+        if (i + N <= count) g[u] = load16<STREAM>(q + i);
+    }
+    if (lane < count % N) {                               // what does not fill a load: an element a lane
+        V last = {};
+        last[0] = q[count / N * N + lane];
+        acc.template take<TYPE>(last);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-        for (int k = 0; k < N; ++k) acc = take<MAX>(acc, Vec<TYPE>::wide(g[u][k]));
-    return acc;
+    for (int u = 0; u < U; ++u) acc.template take<TYPE>(g[u]);
 }
 
-template <bool MAX, int TYPE>
-__device__ __forceinline__ double take_chunk(double acc, const void* p, long long begin, int count)
+// Where a norm comes from and goes, and what the gradients are multiplied by.
+struct Norm {
+    const double* parts; int count, max;       // its parts, or none (count 0) ...
+    const float* given; float* out;            // ... and the norm that the caller has instead; where it is written
+    float max_norm;                            // < 0: no clipping
+};
+
+// The norm from its parts.  Every wave of an update does this for itself, while its loads are under way: 2 KB that its L2 has, and no waiting for other waves.  A launch in between
+// that does it once took 2 to 5 us.
+__device__ __forceinline__ double whole(const Norm& f)
 {
-    return count == CHUNK ? take_chunk<MAX, TYPE, true>(acc, p, begin, count) : take_chunk<MAX, TYPE, false>(acc, p, begin, count);
+    if (f.given) return (double)*f.given;
+    double v[PARTS / 64];
+#pragma unroll
+    for (int k = 0; k < PARTS / 64; ++k) { const int i = k * 64 + (threadIdx.x & 63); v[k] = i < f.count ? f.parts[i] : 0.0; }
+    if (f.max) {
+        Acc<true> acc;
+        for (int k = 0; k < PARTS / 64; ++k) acc.join(v[k]);
+        return Acc<true>::whole(wave_join<true>(acc.part()));
+    }
+    Acc<false> acc;
+    for (int k = 0; k < PARTS / 64; ++k) acc.join(v[k]);
+    return Acc<false>::whole(wave_join<false>(acc.part()));
 }
 
-template <bool MAX>
-__global__ __launch_bounds__(T) void norm_parts_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other,
-                                                       int col, int count, double* __restrict__ parts)
+// min(1, max_norm / (norm + 1e-6)): a NaN norm gives NaN, an infinite one 0, as the quotient does.
+__device__ __forceinline__ float share_of(const Norm& f, double norm)
 {
-    double acc = 0.0;
+    const double s = (double)f.max_norm / (norm + 1e-6);
+    return f.max_norm < 0.f ? 1.f : (float)(s > 1.0 ? 1.0 : s);
+}
+
+struct Hyper { double lr, beta1, beta2, weight_decay; float eps; int decoupled, skip; const float* lr_at; };
+struct Factors { float size, root, keep, had; };               // of one row: lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), 1 - lr decay, the count before
+
+// b^t for a whole number t by squaring, in 64 bits (a count is at most 2^24, where float stops counting): 1 - b^t loses what 32 bits have for small t.
+__device__ __forceinline__ double power(double b, unsigned t)
+{
+    double r = 1.0;
+    for (; t; t >>= 1) { if (t & 1) r *= b; b *= b; }
+    return r;
+}
+
+__device__ __forceinline__ void begin_row(const Row& r, const Hyper& h, Factors* f)
+{
+    const float had = *r.step, t = had + 1.f;
+    const double lr = h.lr_at ? (double)*h.lr_at : h.lr;
+    *r.step = t;
+    *f = {(float)(lr / (1.0 - power(h.beta1, (unsigned)t))), (float)(1.0 / sqrt(1.0 - power(h.beta2, (unsigned)t))), (float)(1.0 - lr * h.weight_decay), had};
+}
+
+__global__ __launch_bounds__(T) void adam_begin_kernel(const Row* __restrict__ rows, int n, Hyper h, Factors* __restrict__ factors)
+{
+    const int k = blockIdx.x * T + threadIdx.x;
+    if (k < n) begin_row(rows[k], h, factors + k);
+}
+
+// One part of the norm for each of the first `sums` workgroups (with one, the norm itself); those behind them, if any, begin a step of Adam.
+template <bool MAX, bool STREAM>
+__global__ __launch_bounds__(TN) void norm_parts_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other,
+                                                        int col, int count, int sums, double* __restrict__ parts, float* __restrict__ out, int n, Hyper h,
+                                                        Factors* __restrict__ factors)
+{
+    if ((int)blockIdx.x >= sums) {
+        const int k = ((int)blockIdx.x - sums) * TN + threadIdx.x;
+        if (k < n) begin_row(rows[k], h, factors + k);
+        return;
+    }
+    constexpr int WAVES = TN / 64;
+    __shared__ double part[WAVES];
+    Acc<MAX> acc;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int c = blockIdx.x * WAVES + wave; c < count; c += gridDim.x * WAVES) {
+    for (int c = blockIdx.x * WAVES + wave; c < count; c += sums * WAVES) {
         const int2 at = chunks[c];
         const Row& r = rows[at.x];
         const void* p = other ? other[at.x] : r.p[col];
         const int type = col ? r.type_g : r.type;
-        const long long begin = (long long)at.y * CHUNK, left = r.n - begin;
-        const int here = left < CHUNK ? (int)left : CHUNK;
-        acc = type == BFSR_LIST_F32 ? take_chunk<MAX, BFSR_LIST_F32>(acc, p, begin, here) : type == BFSR_LIST_F16 ? take_chunk<MAX, BFSR_LIST_F16>(acc, p, begin, here)
-                                                                                                                 : take_chunk<MAX, BFSR_LIST_BF16>(acc, p, begin, here);
+        const long long begin = (long long)at.y * CHUNK;
+        const int here = left_in(r, begin);
+        if (type == BFSR_LIST_F32) take_chunk<MAX, STREAM, BFSR_LIST_F32>(acc, p, begin, here);
+        else if (type == BFSR_LIST_F16) take_chunk<MAX, STREAM, BFSR_LIST_F16>(acc, p, begin, here);
+        else take_chunk<MAX, STREAM, BFSR_LIST_BF16>(acc, p, begin, here);
     }
-    acc = block_join<MAX>(acc);
-    if (threadIdx.x == 0) parts[blockIdx.x] = acc;
-}
-
-struct Final {
-    const double* parts; int count, max;       // the norm's parts, or none (count 0) ...
-    const float* given; float* out;            // ... and the norm that the caller has instead; where it goes
-    float max_norm;                            // < 0: no clipping
-    float* share;                              // what the gradients are multiplied by
-};
-
-// The norm from its parts and the share min(1, max_norm / (norm + 1e-6)), in 64 bits: a NaN norm gives a NaN share, an infinite one 0, as the quotient does.
-__device__ double finish(const Final& f)
-{
-    __shared__ double whole;
-    double v = 0.0;
-    if (f.given) v = (double)*f.given;
-    else {
-        for (int k = threadIdx.x; k < f.count; k += T) v = f.max ? join<true>(v, f.parts[k]) : v + f.parts[k];
-        v = f.max ? block_join<true>(v) : sqrt(block_join<false>(v));
-    }
-    if (threadIdx.x == 0) {
-        whole = v;
-        if (f.out) *f.out = (float)v;
-        if (f.share) {
-            const double s = (double)f.max_norm / (v + 1e-6);
-            *f.share = f.max_norm < 0.f ? 1.f : (float)(s > 1.0 ? 1.0 : s);
+    const double mine = wave_join<MAX>(acc.part());
+    if ((threadIdx.x & 63) == 0) part[wave] = mine;
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        const double all = wave_join<MAX>(threadIdx.x < WAVES ? part[threadIdx.x] : 0.0);
+        if (threadIdx.x == 0) {
+            if (out) *out = (float)Acc<MAX>::whole(all);
+            else parts[blockIdx.x] = all;
         }
     }
-    __syncthreads();
-    return whole;
 }
 
-__global__ __launch_bounds__(T) void norm_finish_kernel(Final f) { finish(f); }
-
-template <bool FULL>
-__device__ __forceinline__ void clip_chunk(const void* from, void* to, int type, int count, float s)
+__global__ __launch_bounds__(64) void norm_finish_kernel(Norm f)
 {
+    const double norm = whole(f);
+    if (threadIdx.x == 0) *f.out = (float)norm;
+}
+
+template <bool STREAM, int TYPE, bool FULL>
+__device__ __forceinline__ void clip_chunk(const Norm& f, const void* from, void* to, int count)
+{
+    typedef typename Vec<TYPE>::type V;
+    constexpr int N = Vec<TYPE>::N, U = CHUNK / (64 * N);
+    const GLOBAL typename Vec<TYPE>::one* p = (const GLOBAL typename Vec<TYPE>::one*)from;
+    GLOBAL typename Vec<TYPE>::one* q = (GLOBAL typename Vec<TYPE>::one*)to;
     const int lane = threadIdx.x & 63;
-    constexpr int U = CHUNK / 256;
-    Four g[U];
+    V g[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) g[u] = load4<FULL>(from, type, (u * 64 + lane) * 4, count);
+    for (int u = 0; u < U; ++u) {
+        const int i = (u * 64 + lane) * N;
+        if (FULL || i + N <= count) g[u] = load16<STREAM>(p + i);
+    }
+    const bool more = !FULL && lane < count % N;                   // what does not fill a load: an element a lane
+    const int last = count / N * N + lane;
+    typename Vec<TYPE>::one e = {};
+    if (more) e = p[last];
+    const double norm = whole(f);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *f.out = (float)norm;
+    const float s = share_of(f, norm);
+    if (s == 1.f && from == to) return;                            // in place, and nothing to change
 #pragma unroll
-    for (int u = 0; u < U; ++u) store4<FULL>(to, type, (u * 64 + lane) * 4, count, floats(g[u], type) * s);
+    for (int u = 0; u < U; ++u) {
+        const int i = (u * 64 + lane) * N;
+#pragma unroll
+        for (int k = 0; k < N; ++k) g[u][k] = Vec<TYPE>::narrow(Vec<TYPE>::wide(g[u][k]) * s);
+        if (FULL || i + N <= count) store16<STREAM>(q + i, g[u]);
+    }
+    if (more) q[last] = Vec<TYPE>::narrow(Vec<TYPE>::wide(e) * s);
 }
 
-__global__ __launch_bounds__(T) void clip_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, int count, const float* __restrict__ share)
+// One chunk for each wave, and then the wave ends: one that went on to another chunk would wait for its stores before the next loads count as arrived.
+// Chunks are taken from the end, where the cache holds what the norm has read last.
+template <bool STREAM>
+__global__ __launch_bounds__(T) void clip_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, int count, Norm f)
 {
-    const int c = blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (c >= count) return;
+    const int c = count - 1 - (int)blockIdx.x * (T / 64) - __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (c < 0) {
+        if (count == 0 && threadIdx.x == 0) *f.out = (float)whole(f);
+        return;
+    }
     const int2 at = chunks[c];
     const Row& r = rows[at.x];
-    const float s = *share;
-    if (s == 1.f && r.p[0] == r.p[1]) return;                  // in place, and nothing to change
-    const long long begin = (long long)at.y * CHUNK, left = r.n - begin;
+    const long long begin = (long long)at.y * CHUNK;
+    const int left = left_in(r, begin);
     const void* from = at_element(r.p[0], r.type, begin);
     void* to = at_element(r.p[1], r.type, begin);
-    if (left >= CHUNK) clip_chunk<true>(from, to, r.type, CHUNK, s);
-    else clip_chunk<false>(from, to, r.type, (int)left, s);
+    const bool full = left == CHUNK;
+    if (r.type == BFSR_LIST_F32) full ? clip_chunk<STREAM, BFSR_LIST_F32, true>(f, from, to, left) : clip_chunk<STREAM, BFSR_LIST_F32, false>(f, from, to, left);
+    else if (r.type == BFSR_LIST_F16) full ? clip_chunk<STREAM, BFSR_LIST_F16, true>(f, from, to, left) : clip_chunk<STREAM, BFSR_LIST_F16, false>(f, from, to, left);
+    else full ? clip_chunk<STREAM, BFSR_LIST_BF16, true>(f, from, to, left) : clip_chunk<STREAM, BFSR_LIST_BF16, false>(f, from, to, left);
 }
 
-struct Hyper { double lr, beta1, beta2, weight_decay; float eps; int decoupled, skip; const float* lr_at; };
-struct Factors { float size, root, keep, go; };                // of one row: lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), 1 - lr decay, whether it is updated
+struct Rule { float b1, c1, b2, c2, wd, eps; bool add, keep, skip; Factors f; };
 
-// One workgroup: the norm, and each row's step count and factors.  Powers and quotients in 64 bits: 1 - beta2^t loses what 32 bits have for small t.
-__global__ __launch_bounds__(T) void adam_begin_kernel(const Row* __restrict__ rows, int n, Final f, Hyper h, Factors* __restrict__ factors)
+__device__ __forceinline__ void adam_element(const Rule& w, float share, float& p, float g, float& m, float& v)
 {
-    double norm = 0.0;
-    if (f.given || f.count) norm = finish(f);
-    else if (threadIdx.x == 0) *f.share = 1.f;
-    const bool go = !(h.skip && !(norm <= 1.7976931348623157e308));
-    const double lr = h.lr_at ? (double)*h.lr_at : h.lr;
-    for (int k = threadIdx.x; k < n; k += T) {
-        const float t = *rows[k].step + 1.f;
-        if (go) *rows[k].step = t;
-        factors[k] = {(float)(lr / (1.0 - pow(h.beta1, (double)t))), (float)(1.0 / sqrt(1.0 - pow(h.beta2, (double)t))),
-                      (float)(1.0 - lr * h.weight_decay), go ? 1.f : 0.f};
-    }
+    float d = g * share;
+    if (w.add) d = fmaf(w.wd, p, d);
+    if (w.keep) p *= w.f.keep;
+    m = fmaf(w.b1, m, w.c1 * d);
+    v = fmaf(w.b2, v, w.c2 * d * d);
+    p -= w.f.size * (m / fmaf(sqrtf(v), w.f.root, w.eps));
 }
 
-struct Rule { float share, b1, c1, b2, c2, wd, eps; bool add, keep; Factors f; };
-
-template <bool FULL>
-__device__ __forceinline__ void adam_chunk(void* pp, const void* gp, float* mp, float* vp, int type, int type_g, int count, const Rule& w)
+template <bool STREAM>
+__device__ __forceinline__ void adam_chunk(const Norm& f, void* pp, const void* gp, float* mp, float* vp, int type, int type_g, int count, const Rule& w)
 {
-    const int lane = threadIdx.x & 63;
-    constexpr int U = 2;
-    for (int j = 0; j < CHUNK && (FULL || j < count); j += U * 256) {
-        Four p[U], g[U], m[U], v[U];
+    constexpr int U = CHUNK / (T * 4), F32 = BFSR_LIST_F32;
+    Four p[U], g[U], m[U], v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = j + (u * 64 + lane) * 4;
-            p[u] = load4<FULL>(pp, type, i, count);
-            g[u] = load4<FULL>(gp, type_g, i, count);
-            m[u] = load4<FULL>(mp, BFSR_LIST_F32, i, count);
-            v[u] = load4<FULL>(vp, BFSR_LIST_F32, i, count);
+    for (int u = 0; u < U; ++u) {
+        const int i = (u * T + threadIdx.x) * 4;
+        if (i + 4 <= count) {
+            p[u] = load4<STREAM>(pp, type, i);
+            g[u] = load4<STREAM>(gp, type_g, i);
+            m[u] = load4<STREAM>(mp, F32, i);
+            v[u] = load4<STREAM>(vp, F32, i);
         }
+    }
+    float share = 1.f;
+    if (f.out) {
+        const double norm = whole(f);
+        if (w.skip && !(norm <= 1.7976931348623157e308)) return;
+        share = share_of(f, norm);
+    }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = j + (u * 64 + lane) * 4;
-            f4 x = floats(p[u], type), y = floats(g[u], type_g), m1, v1;
+    for (int u = 0; u < U; ++u) {
+        const int i = (u * T + threadIdx.x) * 4;
+        if (i + 4 <= count) {
+            f4 x = floats(p[u], type), y = floats(g[u], type_g), m1 = m[u].f, v1 = v[u].f;
+#pragma unroll
             for (int k = 0; k < 4; ++k) {
-                float d = y[k] * w.share;
-                if (w.add) d = fmaf(w.wd, x[k], d);
-                if (w.keep) x[k] *= w.f.keep;
-                m1[k] = fmaf(w.b1, m[u].f[k], w.c1 * d);
-                v1[k] = fmaf(w.b2, v[u].f[k], w.c2 * d * d);
-                x[k] -= w.f.size * (m1[k] / fmaf(sqrtf(v1[k]), w.f.root, w.eps));
+                float a = x[k], b = m1[k], c = v1[k];
+                adam_element(w, share, a, y[k], b, c);
+                x[k] = a; m1[k] = b; v1[k] = c;
             }
-            store4<FULL>(pp, type, i, count, x);
-            store4<FULL>(mp, BFSR_LIST_F32, i, count, m1);
-            store4<FULL>(vp, BFSR_LIST_F32, i, count, v1);
+            store4<STREAM>(pp, type, i, x);
+            store4<STREAM>(mp, F32, i, m1);
+            store4<STREAM>(vp, F32, i, v1);
         }
+    }
+    if ((int)threadIdx.x < (count & 3)) {                          // what does not fill a load
+        const int i = (count & ~3) + threadIdx.x;
+        float a = load1(pp, type, i), b = mp[i], c = vp[i];
+        adam_element(w, share, a, load1(gp, type_g, i), b, c);
+        store1(pp, type, i, a);
+        mp[i] = b;
+        vp[i] = c;
     }
 }
 
-__global__ __launch_bounds__(T) void adam_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other, int count,
-                                                 Hyper h, const Factors* __restrict__ factors, const float* __restrict__ share)
+// One chunk for each workgroup; the last workgroup sees to the norm's output, and to the counts of a step that is skipped.
+template <bool STREAM>
+__global__ __launch_bounds__(T) void adam_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other, int count, int n,
+                                                 Norm f, Hyper h, const Factors* __restrict__ factors)
 {
-    const int c = blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (c >= count) return;
+    const int c = count - 1 - (int)blockIdx.x;
+    if (c < 0) {
+        if (!f.out) return;
+        const double norm = whole(f);
+        if (threadIdx.x == 0) *f.out = (float)norm;
+        if (h.skip && !(norm <= 1.7976931348623157e308))           // infinite or NaN
+            for (int k = threadIdx.x; k < n; k += T) *rows[k].step = factors[k].had;
+        return;
+    }
+    Rule w = {(float)h.beta1, (float)(1.0 - h.beta1), (float)h.beta2, (float)(1.0 - h.beta2), (float)h.weight_decay, h.eps};
+    w.add = w.wd != 0.f && !h.decoupled;
+    w.keep = w.wd != 0.f && h.decoupled;
+    w.skip = h.skip;
     const int2 at = chunks[c];
     const Row& r = rows[at.x];
-    const Factors f = factors[at.x];
-    if (f.go == 0.f) return;
-    const float wd = (float)h.weight_decay;
-    const Rule w = {*share, (float)h.beta1, (float)(1.0 - h.beta1), (float)h.beta2, (float)(1.0 - h.beta2), wd, h.eps, wd != 0.f && !h.decoupled, wd != 0.f && h.decoupled, f};
-    const long long begin = (long long)at.y * CHUNK, left = r.n - begin;
+    w.f = factors[at.x];
+    const long long begin = (long long)at.y * CHUNK;
     void* p = at_element(r.p[0], r.type, begin);
     const void* g = at_element(other ? other[at.x] : r.p[1], r.type_g, begin);
     float* m = (float*)r.p[2] + begin;
     float* v = (float*)r.p[3] + begin;
-    if (left >= CHUNK) adam_chunk<true>(p, g, m, v, r.type, r.type_g, CHUNK, w);
-    else adam_chunk<false>(p, g, m, v, r.type, r.type_g, (int)left, w);
+    adam_chunk<STREAM>(f, p, g, m, v, r.type, r.type_g, left_in(r, begin), w);
 }
 
 // ---- the table: rows and chunks travel to the device as kernel arguments.  No host buffer has to outlive the call, nothing waits for the stream, and a
@@ -348,16 +474,20 @@ __global__ __launch_bounds__(512) void pointer_write_kernel(Pointers all, int n,
     if ((int)threadIdx.x < n) to[threadIdx.x] = all.p[threadIdx.x];
 }
 
-bool good(const BfsrListArgs& a) { return a.rows && a.chunks && a.n > 0 && a.count >= 0 && a.count < (1 << 24) && a.chunk == CHUNK; }
+bool good(const BfsrListArgs& a) { return a.rows && a.chunks && a.n > 0 && a.count >= 0 && a.count < (1 << 24) && a.chunk == CHUNK && a.bytes >= 0; }
 
-int blocks_of(int count) { return (count + WAVES - 1) / WAVES; }
-int parts_of(int count) { return blocks_of(count) < MAX_PARTS ? blocks_of(count) : MAX_PARTS; }
+int sums_of(int count) { const int w = TN / 64, b = (count + w - 1) / w; return count <= ALONE ? 1 : b < PARTS ? b : PARTS; }
 
-int launch_parts(const BfsrListArgs& a, int col, double* parts, hipStream_t st)
+// Whether a call streams its tensors past the cache.
+bool streams(const BfsrListArgs& a) { return a.bytes > CACHE; }
+
+// The parts of a norm; `out`: the norm itself, which one workgroup finds. `h`: with them, the beginning of a step of Adam.
+int launch_parts(const BfsrListArgs& a, int col, bool stream, float* out, const Hyper* h, Factors* factors, hipStream_t st)
 {
-    if (!a.count) return 0;
-    const auto k = a.max ? norm_parts_kernel<true> : norm_parts_kernel<false>;
-    k<<<parts_of(a.count), T, 0, st>>>((const Row*)a.rows, (const int2*)a.chunks, (const void* const*)a.other, col, a.count, parts);
+    const auto k = a.max ? stream ? norm_parts_kernel<true, true> : norm_parts_kernel<true, false> : stream ? norm_parts_kernel<false, true> : norm_parts_kernel<false, false>;
+    const int sums = sums_of(a.count);
+    k<<<sums + (h ? (a.n + TN - 1) / TN : 0), TN, 0, st>>>((const Row*)a.rows, (const int2*)a.chunks, (const void* const*)a.other, col, a.count, sums, (double*)a.work, out, a.n,
+                                                        h ? *h : Hyper{}, factors);
     return (int)hipGetLastError();
 }
 
@@ -365,7 +495,7 @@ int launch_parts(const BfsrListArgs& a, int col, double* parts, hipStream_t st)
 
 extern "C" int bfsr_list_chunk(long long total) { return total < 0 ? -1 : CHUNK; }
 
-extern "C" long long bfsr_list_work(int n) { return n < 0 ? -1 : (long long)MAX_PARTS * 8 + 16 + (long long)n * (long long)sizeof(Factors); }
+extern "C" long long bfsr_list_work(int n) { return n < 0 ? -1 : (long long)PARTS * 8 + (long long)n * (long long)sizeof(Factors); }
 
 extern "C" int bfsr_list_write(const void* const* const* cols, int ncols, const long long* sizes, const int* types, int n, int chunk, void* rows, void* chunks, void* stream)
 {
@@ -406,10 +536,9 @@ extern "C" int bfsr_grad_norm(const BfsrListArgs* a, void* stream)
 {
     if (!a || !good(*a) || !a->work || !a->norm) return -1;
     hipStream_t st = (hipStream_t)stream;
-    double* parts = (double*)a->work;
-    const int err = launch_parts(*a, 0, parts, st);
-    if (err) return err;
-    norm_finish_kernel<<<1, T, 0, st>>>(Final{parts, parts_of(a->count), a->max, nullptr, a->norm, -1.f, nullptr});
+    const int sums = sums_of(a->count), err = launch_parts(*a, 0, streams(*a), sums == 1 ? a->norm : nullptr, nullptr, nullptr, st);
+    if (err || sums == 1) return err;
+    norm_finish_kernel<<<1, 64, 0, st>>>(Norm{(const double*)a->work, sums, a->max, nullptr, a->norm, -1.f});
     return (int)hipGetLastError();
 }
 
@@ -417,12 +546,11 @@ extern "C" int bfsr_clip_grads(const BfsrListArgs* a, float max_norm, void* stre
 {
     if (!a || !good(*a) || !a->work || !a->norm || !(max_norm >= 0.f)) return -1;
     hipStream_t st = (hipStream_t)stream;
-    double* parts = (double*)a->work;
-    float* share = (float*)(parts + MAX_PARTS);
-    const int err = launch_parts(*a, 0, parts, st);
+    const bool past = streams(*a);
+    const int err = launch_parts(*a, 0, past, nullptr, nullptr, nullptr, st), per = T / 64;
     if (err) return err;
-    norm_finish_kernel<<<1, T, 0, st>>>(Final{parts, parts_of(a->count), a->max, nullptr, a->norm, max_norm, share});
-    if (a->count) clip_kernel<<<blocks_of(a->count), T, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, a->count, share);
+    (past ? clip_kernel<true> : clip_kernel<false>)<<<a->count ? (a->count + per - 1) / per : 1, T, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, a->count,
+                                                   Norm{(const double*)a->work, sums_of(a->count), a->max, nullptr, a->norm, max_norm});
     return (int)hipGetLastError();
 }
 
@@ -431,19 +559,20 @@ extern "C" int bfsr_adam_step(const BfsrListArgs* a, const BfsrAdamArgs* h, void
     if (!a || !h || !good(*a) || !a->work) return -1;
     if (!(h->beta1 >= 0. && h->beta1 < 1.) || !(h->beta2 >= 0. && h->beta2 < 1.) || !(h->eps >= 0.f) || !(h->weight_decay >= 0.)) return -1;
     hipStream_t st = (hipStream_t)stream;
-    double* parts = (double*)a->work;
-    float* share = (float*)(parts + MAX_PARTS);
-    Factors* factors = (Factors*)(share + 4);
-    const bool norm = h->max_norm >= 0.f || h->skip_nonfinite;
-    const bool own = norm && !h->given_norm;
+    Factors* factors = (Factors*)((double*)a->work + PARTS);
+    const bool norm = h->max_norm >= 0.f || h->skip_nonfinite, own = norm && !h->given_norm;
     if (norm && !a->norm) return -1;
-    if (own) {
-        const int err = launch_parts(*a, 1, parts, st);
-        if (err) return err;
-    }
     const Hyper hy = {h->lr, h->beta1, h->beta2, h->weight_decay, h->eps, h->decoupled, h->skip_nonfinite, h->lr_at};
-    adam_begin_kernel<<<1, T, 0, st>>>((const Row*)a->rows, a->n, Final{parts, own ? parts_of(a->count) : 0, a->max, norm ? h->given_norm : nullptr, norm ? a->norm : nullptr,
-                                       h->max_norm >= 0.f ? h->max_norm : -1.f, share}, hy, factors);
-    if (a->count) adam_kernel<<<blocks_of(a->count), T, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, (const void* const*)a->other, a->count, hy, factors, share);
+    const bool past = streams(*a);
+    int err;
+    if (own) err = launch_parts(*a, 1, past, nullptr, &hy, factors, st);
+    else {
+        adam_begin_kernel<<<(a->n + T - 1) / T, T, 0, st>>>((const Row*)a->rows, a->n, hy, factors);
+        err = (int)hipGetLastError();
+    }
+    if (err) return err;
+    (past ? adam_kernel<true> : adam_kernel<false>)<<<a->count + 1, T, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, (const void* const*)a->other, a->count, a->n,
+                                                   Norm{(const double*)a->work, own ? sums_of(a->count) : 0, a->max, norm ? h->given_norm : nullptr, norm ? a->norm : nullptr,
+                                                        h->max_norm >= 0.f ? h->max_norm : -1.f}, hy, factors);
     return (int)hipGetLastError();
 }

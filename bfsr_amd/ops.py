@@ -5,7 +5,6 @@ PyTorch is plumbing here (device memory, streams); all arithmetic on the hot pat
 libbfsr_hip.so.  `HipOps` is the only ops backend of the product; tests may substitute a CPU
 test double with the same interface to exercise the host-side schedule without a GPU.
 """
-import contextlib
 import ctypes as C
 import math
 import os
@@ -102,8 +101,8 @@ def _dense(t):
     return True
 
 
-def list_column(tensors, device, what, types=LIST_TYPES, like=None):
-    """`tensors` as a list of aliases without a graph, every one checked: dense memory of one of `types` on `device`; shapes and orders of `like`, tensor by tensor."""
+def list_column(tensors, device, what, types=LIST_TYPES, like=None, alias=True):
+    """`tensors` as a list (of aliases without a graph), every one checked: dense memory of one of `types` on `device`; shapes and orders of `like`, tensor by tensor."""
     if isinstance(tensors, torch.Tensor):
         raise TypeError("%s: need a list of tensors, got one tensor" % what)
     got = list(tensors)
@@ -112,97 +111,139 @@ def list_column(tensors, device, what, types=LIST_TYPES, like=None):
     for k, t in enumerate(got):
         if not isinstance(t, torch.Tensor):
             raise TypeError("%s[%d]: need a tensor, got %s" % (what, k, type(t).__name__))
-        if t.layout != torch.strided or t.dtype not in types or t.device != device:
+        if t.layout is not torch.strided or t.dtype not in types or t.device != device:
             raise ValueError("%s[%d]: need a strided tensor of %s on %s, got %s, %s on %s" % (
                 what, k, " / ".join(str(d)[6:] for d in types), device, t.layout, t.dtype, t.device))
+        if like is not None:
+            same = t.shape == like[k].shape
+            if same and t.stride() == like[k].stride() and not t.is_neg():
+                continue
+            if not same or _order(t) != _order(like[k]):
+                raise ValueError("%s[%d]: shape %s, strides %s do not go with shape %s, strides %s" % (
+                    what, k, tuple(t.shape), t.stride(), tuple(like[k].shape), like[k].stride()))
         if t.is_neg() or not _dense(t):
             raise ValueError("%s[%d]: not dense memory (shape %s, strides %s)" % (what, k, tuple(t.shape), t.stride()))
-        if like is not None and (t.shape != like[k].shape or _order(t) != _order(like[k])):
-            raise ValueError("%s[%d]: shape %s, strides %s do not go with shape %s, strides %s" % (
-                what, k, tuple(t.shape), t.stride(), tuple(like[k].shape), like[k].stride()))
-    return [t.detach() for t in got]
+    return [t.detach() for t in got] if alias else got
+
+
+def _versions(tensors):
+    """Of `tensors`, one for each version counter: views of one tensor share it, and there may be hundreds of them."""
+    bases, got = set(), []
+    for t in tensors:
+        base = t._base
+        if base is not None:
+            if id(base) in bases:
+                continue
+            bases.add(id(base))
+        if not t.is_inference():
+            got.append(t.detach())
+    return got
+
+
+def _addresses(tensors):
+    return np.array([t.data_ptr() for t in tensors], dtype=np.int64)
+
+
+def _bytes(tensors):
+    return np.array([t.nbytes for t in tensors], dtype=np.int64)
 
 
 class Spans(object):
-    """The pieces of memory that tensors take, sorted; they may not overlap."""
+    """Pieces of memory (addresses and bytes; 0 bytes are none), sorted; they may not overlap."""
 
-    def __init__(self, tensors, what):
-        live = [(t.data_ptr(), t.numel() * t.element_size()) for t in tensors if t.numel()]
-        a = np.array(live, dtype=np.int64).reshape(-1, 2)
-        a = a[np.argsort(a[:, 0], kind="stable")]
-        self.start, self.end = a[:, 0], a[:, 0] + a[:, 1]
+    def __init__(self, at, size, what):
+        if not size.all():
+            at, size = at[size > 0], size[size > 0]
+        by = np.argsort(at, kind="stable")
+        self.start = at[by]
+        self.end = self.start + size[by]
         if (self.start[1:] < self.end[:-1]).any():
             raise ValueError("%s: two of the tensors that are written overlap (or one is there twice)" % what)
 
-    def meet(self, tensors):
-        """Whether one of `tensors` overlaps one of these."""
-        live = [(t.data_ptr(), t.numel() * t.element_size()) for t in tensors if t.numel()]
-        if not live or not self.start.size:
+    def meet(self, at, size):
+        """Whether one of the given pieces overlaps one of these."""
+        if not self.start.size:
             return False
-        a = np.array(live, dtype=np.int64)
-        k = np.searchsorted(self.end, a[:, 0], side="right")           # the first piece that ends behind the tensor's start
+        k = np.searchsorted(self.end, at, side="right")                # the first piece that ends behind the other's start
         near = np.minimum(k, self.start.size - 1)
-        return bool(((k < self.start.size) & (self.start[near] < a[:, 0] + a[:, 1])).any())
+        return bool(((k < self.start.size) & (size > 0) & (self.start[near] < at + size)).any())
 
 
 class ListTable(object):
-    """The device table of a list of tensors (HipOps.tensor_list, HipOps.adam).  It names the memory that the tensors had when it was made, and holds on to it."""
+    """The device table of a list of tensors (HipOps.tensor_list, HipOps.adam).  It names the memory that the tensors had when it was made.
 
-    def __init__(self, ops, cols, types, once):
-        self.ops, self.n, self.once = ops, len(cols[0]), once
-        self.sizes = [t.numel() for t in cols[0]]
-        self.chunk = ops.lib.bfsr_list_chunk(sum(self.sizes))
-        self.count = sum(-(-s // self.chunk) for s in self.sizes)
+    `cols`: the addresses of each column, `sizes`: elements, `types`: types of the rows, `nbytes`: of all tensors, each once."""
+
+    def __init__(self, ops, cols, sizes, types, nbytes, once):
+        self.ops, self.n, self.once, self.bytes = ops, len(types), once, int(nbytes)
+        self.chunk = ops.lib.bfsr_list_chunk(int(sizes.sum()))
+        self.count = int(((sizes + (self.chunk - 1)) // self.chunk).sum())
         if self.count >= 1 << 24:
-            raise ValueError("tensor list: %d elements are too many for one list" % sum(self.sizes))
+            raise ValueError("tensor list: %d elements are too many for one list" % sizes.sum())
+        self.device = ops._index_device()
         self.stream, self.table = None, None
         if not self.n:
             return
-        dev = ops._index_device()
-        with torch.cuda.device(dev):
+        self.work = ops.lib.bfsr_list_work(self.n) // 8
+        types = np.array(types, dtype=np.int32)
+        with torch.cuda.device(self.device):
             if not once and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("tensor list: make it before the capture begins (its table is written once, not at every replay)")
-            stream = torch.cuda.current_stream(dev)
+            stream = torch.cuda.current_stream(self.device)
             self.stream = stream.cuda_stream
-            self.table = torch.empty(self.n * 8 + max(self.count, 1), dtype=torch.int64, device=dev)
-            n = self.n
-            held = [(C.c_void_p * n)(*[t.data_ptr() for t in c]) for c in cols]
-            ptrs = (C.c_void_p * len(cols))(*[C.addressof(h) for h in held])
-            _lib.check(ops.lib.bfsr_list_write(ptrs, len(cols), (C.c_longlong * n)(*self.sizes), (C.c_int * n)(*types), n, self.chunk,
-                                               self.table.data_ptr(), self.table.data_ptr() + 64 * n, C.c_void_p(self.stream)), "list_write")
+            self.table = torch.empty(self.n * 8 + max(self.count, 1), dtype=torch.int64, device=self.device)
+            self.rows = self.table.data_ptr()
+            self.chunks = self.rows + 64 * self.n
+            cols = [np.ascontiguousarray(c) for c in cols]
+            ptrs = (C.c_void_p * len(cols))(*[c.ctypes.data for c in cols])
+            _lib.check(ops.lib.bfsr_list_write(ptrs, len(cols), sizes.ctypes.data, types.ctypes.data, self.n, self.chunk, self.rows, self.chunks, self.stream),
+                       "list_write")
             if not once:
                 stream.synchronize()               # from here on the table may be read on any stream
 
-    def args(self, ops, norm_type, norm):
-        """The C arguments of one call on the current stream, and that stream."""
-        stream = torch.cuda.current_stream(ops._index_device())
+    def call(self, name, fn, kind, norm, *more, grads=None):
+        """One C call over the list on the current stream; `grads`: addresses in place of the table's gradients."""
+        i = self.device.index
+        if torch.cuda.current_device() != i:       # a launch needs its device to be the current one
+            with torch.cuda.device(i):
+                return self.call(name, fn, kind, norm, *more, grads=grads)
+        ops, stream = self.ops, torch._C._cuda_getCurrentRawStream(i)
         if self.once:
-            if stream.cuda_stream != self.stream:
+            if stream != self.stream:
                 raise RuntimeError("tensor list: one made with once=True belongs to the stream it was made on")
         else:
-            if stream.cuda_stream != self.stream:
-                self.table.record_stream(stream)
+            if stream != self.stream:
+                self.table.record_stream(torch.cuda.current_stream(i))
             if torch.cuda.is_current_stream_capturing():
-                ops._captured_tables.append(self.table)      # a graph reads it at every replay, whatever becomes of the list
-        a = _lib.BfsrListArgs()
-        a.rows = self.table.data_ptr()
-        a.chunks = a.rows + 64 * self.n
-        a.n, a.count, a.chunk, a.max = self.n, self.count, self.chunk, int(norm_type == math.inf)
-        work = torch.empty(ops.lib.bfsr_list_work(self.n) // 8, dtype=torch.float64, device=self.table.device)
-        a.work = work.data_ptr()
-        if norm is not None:
-            a.norm = norm.data_ptr()
-        return a, stream, work
+                ops._captured_tables[id(self.table)] = self.table      # a graph reads it at every replay, whatever becomes of the list
+        other = None
+        if grads is not None:
+            other = torch.empty(self.n, dtype=torch.int64, device=self.device)
+            _lib.check(ops.lib.bfsr_pointer_write(grads.ctypes.data, self.n, other.data_ptr(), stream), "pointer_write")
+        work = torch.empty(self.work, dtype=torch.float64, device=self.device)
+        a = _lib.BfsrListArgs(self.rows, self.chunks, self.n, self.count, self.chunk, kind, _ptr(other), self.bytes, work.data_ptr(), _ptr(norm))
+        if ops._keylog is None and ops.profile_keys is None:
+            err = fn(a, *more, stream)
+        else:
+            err = ops._launch((name, self.n, self.count), lambda: fn(a, *more, stream))
+        if err:
+            _lib.check(err, name)
+
+
+_NORMS = {2.0: 0, math.inf: 1, "inf": 1}
 
 
 def _norm_type(v):
-    v = math.inf if v == "inf" else float(v)
-    if v not in (2.0, math.inf):
-        raise ValueError("norm_type: 2 or inf, got %r" % v)
-    return v
+    """The kernels' number of a norm."""
+    kind = _NORMS.get(v)
+    if kind is None:
+        raise ValueError("norm_type: 2 or inf, got %r" % (v,))
+    return kind
 
 
 def _at_least_0(v, what, below=math.inf):
+    if isinstance(v, torch.Tensor):
+        raise TypeError("%s: need a number, got a tensor" % what)
     v = float(v)
     if not 0.0 <= v <= below or (below == 1.0 and v == 1.0):
         raise ValueError("%s: %r is out of range" % (what, v))
@@ -220,16 +261,23 @@ class TensorList(ListTable):
 
     def __init__(self, ops, tensors, out=None, once=False):
         dev = ops._index_device()
-        self.tensors = list_column(tensors, dev, "tensor_list")
-        self.out = None
-        if out is not None:
-            self.out = list_column(out, dev, "tensor_list.out", like=self.tensors)
-            if any(a.dtype != b.dtype for a, b in zip(self.tensors, self.out)):
+        tensors = list_column(tensors, dev, "tensor_list", alias=False)
+        at, nbytes = _addresses(tensors), _bytes(tensors)
+        # aliases hold the memory that the table names, whatever becomes of the tensors
+        self.tensors, self.out, cols = [t.detach() for t in tensors], None, [at]
+        if out is None:
+            Spans(at, nbytes, "tensor_list")
+        else:
+            out = list_column(out, dev, "tensor_list.out", like=tensors, alias=False)
+            self.out = [t.detach() for t in out]
+            if any(a.dtype != b.dtype for a, b in zip(tensors, out)):
                 raise ValueError("tensor_list.out: need the types of the tensors")
-        if Spans(self.tensors if out is None else self.out, "tensor_list").meet(self.tensors if out is not None else []):
-            raise ValueError("tensor_list.out: overlaps the tensors (leave `out` away to write in place)")
-        self.written = [t for t in (self.tensors if out is None else self.out) if not t.is_inference()]
-        super().__init__(ops, [self.tensors] if out is None else [self.tensors, self.out], [LIST_TYPES[t.dtype] for t in self.tensors], once)
+            cols.append(_addresses(out))
+            if Spans(cols[1], nbytes, "tensor_list.out").meet(at, nbytes):
+                raise ValueError("tensor_list.out: overlaps the tensors (leave `out` away to write in place)")
+        self.written = _versions(tensors if out is None else out)
+        sizes = np.array([t.numel() for t in tensors], dtype=np.int64)
+        super().__init__(ops, cols, sizes, [LIST_TYPES[t.dtype] for t in tensors], nbytes.sum() * len(cols), once)
 
 
 class AdamPlan(ListTable):
@@ -237,26 +285,45 @@ class AdamPlan(ListTable):
 
     def __init__(self, ops, params, grads, exp_avg, exp_avg_sq, step):
         dev, f32 = ops._index_device(), {torch.float32: 0}
-        self.params = list_column(params, dev, "adam.params")
-        if not self.params:
+        params = list_column(params, dev, "adam.params", alias=False)
+        if not params:
             raise ValueError("adam: the list of parameters is empty")
-        self.grads = None if grads is None else list_column(grads, dev, "adam.grads", like=self.params)
-        self.grad_types = [t.dtype for t in (self.grads or self.params)]
-        self.exp_avg = list_column(exp_avg, dev, "adam.exp_avg", f32, like=self.params)
-        self.exp_avg_sq = list_column(exp_avg_sq, dev, "adam.exp_avg_sq", f32, like=self.params)
+        self.params = [t.detach() for t in params]
+        self.grads = None if grads is None else list_column(grads, dev, "adam.grads", like=params)
+        self.exp_avg = list_column(exp_avg, dev, "adam.exp_avg", f32, like=params)
+        self.exp_avg_sq = list_column(exp_avg_sq, dev, "adam.exp_avg_sq", f32, like=params)
         if isinstance(step, torch.Tensor):
             if step.dim() != 1:
                 raise ValueError("adam.step: need a 1-d tensor, or a list of tensors of one float32")
             step = step.unbind()
         self.step = [_one_float(t, dev, "adam.step").detach() for t in step]
-        if len(self.step) != len(self.params):
-            raise ValueError("adam.step: %d counts for %d parameters" % (len(self.step), len(self.params)))
-        self.spans = Spans(self.params + self.exp_avg + self.exp_avg_sq + self.step, "adam")
-        if self.spans.meet(self.grads or []):
+        if len(self.step) != len(params):
+            raise ValueError("adam.step: %d counts for %d parameters" % (len(self.step), len(params)))
+        grad_types = [t.dtype for t in (self.grads or params)]
+        self.expect = [(d, t.shape, t.stride()) for d, t in zip(grad_types, params)]      # of a gradient
+        sizes = np.array([t.numel() for t in params], dtype=np.int64)
+        self.grad_bytes = sizes * np.array([d.itemsize for d in grad_types])
+        at = [_addresses(c) for c in (self.params, self.exp_avg, self.exp_avg_sq, self.step)]
+        size = [_bytes(params), sizes * 4, sizes * 4, np.full_like(sizes, 4)]
+        self.spans = Spans(np.concatenate(at), np.concatenate(size), "adam")
+        grad_at = at[0] if grads is None else _addresses(self.grads)
+        if grads is not None and self.spans.meet(grad_at, self.grad_bytes):
             raise ValueError("adam.grads: overlap what the update writes")
-        self.written = [t for t in self.params if not t.is_inference()]
-        super().__init__(ops, [self.params, self.grads or self.params, self.exp_avg, self.exp_avg_sq, self.step],
-                         [LIST_TYPES[p.dtype] | LIST_TYPES[g] << 4 for p, g in zip(self.params, self.grad_types)], False)
+        self.written = _versions(params)
+        super().__init__(ops, [at[0], grad_at] + at[1:], sizes, [LIST_TYPES[p.dtype] | LIST_TYPES[g] << 4 for p, g in zip(params, grad_types)],
+                         self.grad_bytes.sum() + sum(n.sum() for n in size), False)
+
+    def fit(self, grads):
+        """The addresses of a step's gradients, or None where one of them is not what the plan expects."""
+        dev = self.device.index
+        if len(grads) != self.n:
+            return None
+        for g, (dtype, shape, stride) in zip(grads, self.expect):
+            if not isinstance(g, torch.Tensor) or g.layout is not torch.strided or g.dtype is not dtype or g.get_device() != dev or g.shape != shape or g.is_neg():
+                return None
+            if g.stride() != stride and not (_dense(g) and _order(g) == tuple(s for s, n in zip(stride, shape) if n != 1 and g.numel())):
+                return None
+        return _addresses(grads)
 
     def run(self, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled=False, max_norm=None, norm_type=2.0, grad_norm=None, skip_nonfinite=False, grads=None):
         """One step: the counts go up by one, moments and parameters are updated in place.  Nothing waits for the device; may be captured.
@@ -270,42 +337,35 @@ class AdamPlan(ListTable):
                           parameters, types of the plan's gradients)
 
         Returns the norm before clipping (0-d, on the device) with max_norm or skip_nonfinite, None otherwise."""
-        ops = self.ops
-        dev = ops._index_device()
-        h = _lib.BfsrAdamArgs()
+        at = None
+        if grads is not None:
+            at = self.fit(grads)
+            if at is None:
+                raise ValueError("adam.grads: need tensors of the plan's gradients' types, on its device, in the parameters' shapes and orders of axes")
+        elif self.grads is None:
+            raise ValueError("adam.grads: the plan was made without gradients, so run() needs them")
+        return self._run(at, lr, betas, eps, weight_decay, decoupled, max_norm, norm_type, grad_norm, skip_nonfinite)
+
+    def _run(self, grads, lr, betas, eps, weight_decay, decoupled, max_norm, norm_type, grad_norm, skip_nonfinite):
+        """run() with the addresses that fit() gave, or None."""
+        dev, at = self.device, None
         if isinstance(lr, torch.Tensor):
-            h.lr_at = _one_float(lr, dev, "adam.lr").data_ptr()
-        else:
-            h.lr = _at_least_0(lr, "adam.lr")
-        h.beta1, h.beta2 = (_at_least_0(b, "adam.betas", 1.0) for b in betas)
-        h.eps, h.weight_decay = _at_least_0(eps, "adam.eps"), _at_least_0(weight_decay, "adam.weight_decay")
-        h.decoupled, h.skip_nonfinite = int(bool(decoupled)), int(bool(skip_nonfinite))
-        h.max_norm = -1.0 if max_norm is None else _at_least_0(max_norm, "adam.max_norm")
-        norm_type = _norm_type(norm_type)
-        norm = None
+            at, lr = _one_float(lr, dev, "adam.lr").data_ptr(), 0.0
+        beta1, beta2 = betas
+        kind = _norm_type(norm_type)
+        norm = given = None
         if max_norm is not None or skip_nonfinite:
             norm = torch.empty((), dtype=torch.float32, device=dev)
             if grad_norm is not None:
-                h.given_norm = _one_float(grad_norm, dev, "adam.grad_norm").data_ptr()
+                given = _one_float(grad_norm, dev, "adam.grad_norm").data_ptr()
         elif grad_norm is not None:
             raise ValueError("adam.grad_norm: goes with max_norm or skip_nonfinite")
-        if grads is None:
-            if self.grads is None:
-                raise ValueError("adam.grads: the plan was made without gradients, so run() needs them")
-        else:
-            grads = list_column(grads, dev, "adam.grads", like=self.params)
-            if any(g.dtype != t for g, t in zip(grads, self.grad_types)):
-                raise ValueError("adam.grads: need the types of the plan's gradients")
-            if self.spans.meet(grads):
-                raise ValueError("adam.grads: overlap what the update writes")
-        with ops._on_device():
-            a, stream, work = self.args(ops, norm_type, norm)
-            st = C.c_void_p(stream.cuda_stream)
-            if grads is not None:
-                other = torch.empty(self.n, dtype=torch.int64, device=dev)
-                _lib.check(ops.lib.bfsr_pointer_write((C.c_void_p * self.n)(*[g.data_ptr() for g in grads]), self.n, other.data_ptr(), st), "pointer_write")
-                a.other = other.data_ptr()
-            _lib.check(ops._launch(("adam_step", self.n, self.count), lambda: ops.lib.bfsr_adam_step(C.byref(a), C.byref(h), st)), "adam_step")
+        h = _lib.BfsrAdamArgs(_at_least_0(lr, "adam.lr"), at, _at_least_0(beta1, "adam.betas", 1.0), _at_least_0(beta2, "adam.betas", 1.0),
+                              _at_least_0(weight_decay, "adam.weight_decay"), _at_least_0(eps, "adam.eps"), bool(decoupled),
+                              -1.0 if max_norm is None else _at_least_0(max_norm, "adam.max_norm"), given, bool(skip_nonfinite))
+        if grads is not None and self.spans.meet(grads, self.grad_bytes):
+            raise ValueError("adam.grads: overlap what the update writes")
+        self.call("adam_step", self.ops.lib.bfsr_adam_step, kind, norm, h, grads=grads)
         torch.autograd.graph.increment_version(self.written)
         return norm
 
@@ -343,7 +403,7 @@ class HipOps(object):
         self.range_flag = torch.zeros(1, dtype=torch.int32, device=self.device)
         # guard.run_guarded: passes re-run under the bf16x3 split because the fp16 pair met a value outside its range (0 in normal operation)
         self.fallbacks, self._fallback, self._guard_depth, self._range_scratch = 0, None, 0, None
-        self._captured_tables = []                       # tables of tensor lists that captured graphs read
+        self._captured_tables = {}                       # tables of tensor lists that captured graphs read
 
     def cu_count(self):
         """Compute units of the device (the persistent kernels launch one workgroup per CU)."""
@@ -383,11 +443,6 @@ class HipOps(object):
         d = self.device
         return d if d.index is not None else torch.device(d.type, torch.cuda.current_device())
 
-    def _on_device(self):
-        """A launch needs its device to be the current one."""
-        i = self.device.index
-        return contextlib.nullcontext() if i is None or i == torch.cuda.current_device() else torch.cuda.device(i)
-
     # ---- lists of tensors: the end of a training step ------------------------------------------
     def tensor_list(self, tensors, out=None, once=False):
         """A handle of a list of gradients for grad_norm and clip_grads: dense float32 / float16 / bfloat16 tensors on this device, in any mixture, order of
@@ -401,31 +456,24 @@ class HipOps(object):
     def grad_norm(self, tensors, norm_type=2.0, out=None):
         """The norm of all elements of a tensor_list: 2 (summed in 64 bits, so finite gradients have a finite norm as far as float32 holds it) or inf.
         NaN where an element is.  Returns a 0-d float32 on the device (`out`, if given)."""
-        norm_type = _norm_type(norm_type)
-        norm = self._norm_out(tensors, out)
+        kind, norm = _norm_type(norm_type), self._norm_out(tensors, out)
         if tensors.n:
-            with self._on_device():
-                a, stream, work = tensors.args(self, norm_type, norm)
-                _lib.check(self._launch(("grad_norm", tensors.n, tensors.count), lambda: self.lib.bfsr_grad_norm(C.byref(a), C.c_void_p(stream.cuda_stream))), "grad_norm")
+            tensors.call("grad_norm", self.lib.bfsr_grad_norm, kind, norm)
         return norm
 
     def clip_grads(self, tensors, max_norm, norm_type=2.0):
         """Multiplies a tensor_list by min(1, max_norm / (norm + 1e-6)), in place or into its `out`; returns the norm before (0-d float32, on the device).
         An infinite norm makes finite gradients 0, a NaN makes all NaN, as the quotient does.  Products are rounded once, to the tensor's type."""
-        norm_type, max_norm = _norm_type(norm_type), _at_least_0(max_norm, "clip_grads.max_norm")
-        norm = self._norm_out(tensors, None)
+        kind, max_norm, norm = _norm_type(norm_type), _at_least_0(max_norm, "clip_grads.max_norm"), self._norm_out(tensors, None)
         if tensors.n:
-            with self._on_device():
-                a, stream, work = tensors.args(self, norm_type, norm)
-                _lib.check(self._launch(("clip_grads", tensors.n, tensors.count),
-                                        lambda: self.lib.bfsr_clip_grads(C.byref(a), max_norm, C.c_void_p(stream.cuda_stream))), "clip_grads")
+            tensors.call("clip_grads", self.lib.bfsr_clip_grads, kind, norm, max_norm)
             torch.autograd.graph.increment_version(tensors.written)
         return norm
 
     def _norm_out(self, tensors, out):
         if not isinstance(tensors, TensorList) or tensors.ops is not self:
             raise TypeError("need a handle from this object's tensor_list()")
-        dev = self._index_device()
+        dev = tensors.device
         if out is not None:
             _one_float(out, dev, "grad_norm.out")
             return out if tensors.n else out.zero_()

@@ -92,16 +92,24 @@ class Adam(torch.optim.Optimizer):
         return [self.state[p] for p in params]
 
     def _plan(self, at, ops, params, grads):
-        """The group's plan, if it still names the memory that parameters and state have, or a new one."""
+        """The group's plan, if it still names the memory that parameters and state have, or a new one; the gradients in its order of axes, and where they are."""
         state = self._state_of(params)
-        cols = [params] + [[s[k] for s in state] for k in ("exp_avg", "exp_avg_sq", "step")]
-        where = [t.data_ptr() for c in cols for t in c]
-        kinds = [g.dtype for g in grads]
+        where = [t.data_ptr() for t in params]
+        for name in ("exp_avg", "exp_avg_sq", "step"):
+            where += [s[name].data_ptr() for s in state]
         held = self._plans.get(at)
-        if held is None or held[0] is not ops or held[1] != where or held[2] != kinds:
-            bring = all(k == p.dtype for k, p in zip(kinds, params))         # the plan holds no gradients, which zero_grad may want to free
-            held = self._plans[at] = (ops, where, kinds, ops.adam(cols[0], None if bring else grads, *cols[1:]))
-        return held[3]
+        if held is not None and (held[0] is not ops or held[1] != where):
+            held = None
+        found = None if held is None else held[2].fit(grads)
+        if found is None:
+            grads = [g if _order(g) == _order(p) else torch.empty_like(p, dtype=g.dtype).copy_(g) for p, g in zip(params, grads)]
+            found = None if held is None else held[2].fit(grads)
+        if found is None:
+            bring = all(g.dtype == p.dtype for p, g in zip(params, grads))       # the plan holds no gradients, which zero_grad may want to free
+            plan = ops.adam(params, None if bring else grads, *[[s[k] for s in state] for k in ("exp_avg", "exp_avg_sq", "step")])
+            held, found = (ops, where, plan), plan.fit(grads)
+            self._plans[at] = held
+        return held[2], grads, found
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -111,25 +119,27 @@ class Adam(torch.optim.Optimizer):
                 loss = closure()
         work = []
         for at, group in enumerate(self.param_groups):
-            params = [p for p in group["params"] if p.grad is not None]
-            if not params:
-                continue
-            grads = []
-            for p in params:
-                g = p.grad
-                if g.is_sparse:
-                    raise RuntimeError("Adam: sparse gradients are not supported")
-                grads.append(g if _order(g) == _order(p) else torch.empty_like(p, dtype=g.dtype).copy_(g))
-            ops = self._ops or _ops_of(params[0])
-            work.append((group, self._plan(at, ops, params, grads), grads, ops))
+            params = group["params"]
+            grads = [p.grad for p in params]
+            if any(g is None for g in grads):
+                params = [p for p, g in zip(params, grads) if g is not None]
+                grads = [g for g in grads if g is not None]
+            if any(g.is_sparse for g in grads):
+                raise RuntimeError("Adam: sparse gradients are not supported")
+            if params:
+                ops = self._ops or _ops_of(params[0])
+                work.append((group, *self._plan(at, ops, params, grads)))
         self.grad_norm = None
         wants = self.max_grad_norm is not None or self.skip_nonfinite
         norm = None
         if wants and len(work) > 1:
-            ops = work[0][3]
+            ops = work[0][1].ops
             norm = ops.grad_norm(ops.tensor_list([g for w in work for g in w[2]], once=True))
-        for group, plan, grads, ops in work:
-            got = plan.run(group["lr"], group["betas"], group["eps"], group["weight_decay"], group["decoupled_weight_decay"], self.max_grad_norm,
-                           grad_norm=norm, skip_nonfinite=self.skip_nonfinite, grads=grads)
+        for group, plan, _, found in work:
+            lr = group["lr"]
+            if isinstance(lr, torch.Tensor) and lr.device.type == "cpu":
+                lr = float(lr)
+            got = plan._run(found, lr, group["betas"], group["eps"], group["weight_decay"], group["decoupled_weight_decay"], self.max_grad_norm, 2.0, norm,
+                            self.skip_nonfinite)
             self.grad_norm = got if norm is None else norm
         return loss

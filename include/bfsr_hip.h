@@ -613,6 +613,7 @@ typedef struct BfsrListArgs {
     int n, count, chunk;                     /* rows, chunks, elements a chunk */
     int max;                                 /* the norm: 0 Euclidean, 1 the largest magnitude */
     const void* other;                       /* bfsr_adam_step: NULL, or the gradients' n pointers in place of the table's (same sizes and types) */
+    long long bytes;                         /* of all tensors that the call reads or writes, each once: what is larger than the cache streams past it */
     void* work;                              /* scratch of this call alone, bfsr_list_work(n) bytes, 16-byte aligned */
     float* norm;                             /* where the norm goes (bfsr_adam_step: only with max_norm >= 0 or skip_nonfinite) */
 } BfsrListArgs;

@@ -52,20 +52,22 @@ def test_list_column_takes_any_dense_order():
 
 def test_spans_find_overlaps():
     a = torch.zeros(100)
-    O.Spans([a[:10], a[10:20], a[50:], a[30:30], a[20:50]], "x")
+    pieces = lambda ts: (O._addresses(ts), O._bytes(ts))                    # noqa: E731
+    spans = lambda ts: O.Spans(*pieces(ts), "x")                            # noqa: E731
+    spans([a[:10], a[10:20], a[50:], a[30:30], a[20:50]])
     for pair in ([a, a], [a[:10], a[9:20]], [a, a[40:41]], [a[5:6], a[:10]]):
         with pytest.raises(ValueError):
-            O.Spans(pair, "x")
-    s = O.Spans([a[10:20], a[40:60]], "x")
-    assert not s.meet([]) and not s.meet([a[:10], a[20:40], a[60:], a[15:15]])
+            spans(pair)
+    s = spans([a[10:20], a[40:60]])
+    assert not s.meet(*pieces([])) and not s.meet(*pieces([a[:10], a[20:40], a[60:], a[15:15]]))
     for t in (a[9:11], a[19:25], a[30:41], a[59:], a[12:13], a):
-        assert s.meet([a[:5], t])
-    assert not O.Spans([], "x").meet([a])
+        assert s.meet(*pieces([a[:5], t]))
+    assert not spans([]).meet(*pieces([a]))
 
 
 def test_numbers_out_of_range_are_refused():
-    assert O._norm_type("inf") == math.inf and O._norm_type(2) == 2.0
-    for v in (1.0, 0, -1, math.nan, 3.5):
+    assert O._norm_type("inf") == O._norm_type(math.inf) == 1 and O._norm_type(2) == O._norm_type(2.0) == 0
+    for v in (1.0, 0, -1, math.nan, 3.5, None):
         with pytest.raises(ValueError):
             O._norm_type(v)
     for v in (-1e-30, math.nan, -math.inf):
@@ -73,6 +75,8 @@ def test_numbers_out_of_range_are_refused():
             O._at_least_0(v, "x")
     with pytest.raises(ValueError):
         O._at_least_0(1.0, "beta", 1.0)
+    with pytest.raises(TypeError):
+        O._at_least_0(torch.ones(()), "x")
     assert O._at_least_0(0.999, "beta", 1.0) == 0.999 and O._at_least_0(math.inf, "x") == math.inf
     for t in (torch.zeros(2), torch.zeros((), dtype=torch.float64), 1.0, torch.zeros((), device="meta")):
         with pytest.raises(ValueError):
@@ -82,7 +86,7 @@ def test_numbers_out_of_range_are_refused():
 def test_c_entries_refuse_before_a_launch():
     lib = _lib.load()
     chunk = lib.bfsr_list_chunk(1000)
-    assert chunk > 0 and chunk % 1024 == 0 and lib.bfsr_list_chunk(-1) == -1 and lib.bfsr_list_work(-1) == -1 and lib.bfsr_list_work(5) > 8192
+    assert chunk > 0 and chunk % 1024 == 0 and lib.bfsr_list_chunk(-1) == -1 and lib.bfsr_list_work(-1) == -1 and lib.bfsr_list_work(5) > lib.bfsr_list_work(0) > 0
     one = (C.c_void_p * 1)(4096)
     cols = lambda n: (C.c_void_p * n)(*[C.addressof(one)] * n)             # noqa: E731
     size, kind = (C.c_longlong * 1)(8), (C.c_int * 1)(0)
@@ -183,6 +187,13 @@ def test_train_step_clips_with_the_models_ops(golden_dir):
 
 # ---- GPU --------------------------------------------------------------------------------------------------------------------------------
 gpu = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _grad():
+    """Other test modules turn gradients off for the whole process."""
+    with torch.enable_grad():
+        yield
 
 
 @pytest.fixture(scope="module")
@@ -745,3 +756,20 @@ def test_train_step_on_the_gpu(hip, golden_dir):
         first = 0.01 * (g * share) / ((g * share).abs() + 1e-8)                     # Adam's first step
         big = g.abs() > 1e-3 * g.abs().max()
         assert ((a.detach() - b.detach()).cpu().double() - first)[big].abs().max() <= 1e-5
+
+
+@gpu
+def test_versions_of_views_and_plain_tensors(hip):
+    """In-place results count as changes of what they are seen through, once a call."""
+    base = torch.ones(100, device="cuda:0")
+    views, plain = [base[:10], base[20:50].view(5, 6)], torch.ones(7, device="cuda:0")
+    leaf = torch.nn.Parameter(torch.ones(8, device="cuda:0"))
+    before = base._version, plain._version, leaf._version
+    hip.clip_grads(hip.tensor_list(views + [plain, leaf]), 0.5)
+    assert (base._version, plain._version, leaf._version) == tuple(v + 1 for v in before) and views[1]._version == base._version
+    with torch.enable_grad():
+        y = (leaf * leaf).sum()
+    zeros = [torch.zeros(8, device="cuda:0") for _ in range(2)]
+    hip.adam([leaf], [torch.ones(8, device="cuda:0")], zeros[:1], zeros[1:], torch.zeros(1, device="cuda:0")).run(0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
