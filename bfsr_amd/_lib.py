@@ -287,6 +287,7 @@ SYMBOLS = {
     "bfsr_channel_range_check": (_I, [_VP, _LL, _I, _I, _I, _I, _F, _F, _F, _VP, _VP, _VP, _VP]),
     "bfsr_list_chunk": (_I, [_LL]),
     "bfsr_list_work": (_LL, [_I]),
+    "bfsr_norm_work": (_LL, [_I]),
     "bfsr_list_write": (_I, [_VP, _I, _VP, _VP, _I, _I, _VP, _VP, _VP]),
     "bfsr_pointer_write": (_I, [_VP, _I, _VP, _VP]),
     "bfsr_grad_norm": (_I, [C.POINTER(BfsrListArgs), _VP]),

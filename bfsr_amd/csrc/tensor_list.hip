@@ -19,8 +19,13 @@ constexpr int T = 256;                        // threads of a workgroup that upd
 constexpr int TN = 1024;                      // threads of one that sums
 constexpr int CHUNK = 2048;                   // elements of a chunk
 constexpr int PARTS = 256;                    // partial results of a norm at most, one for each of its workgroups: one a CU, and four a lane for the wave that joins them
-constexpr int ALONE = 16;                     // chunks up to which one workgroup sums a list by itself
-constexpr long long CACHE = 128ll << 20;      // bytes of tensors up to which a call counts on finding, and leaves, them in the 256 MB cache that the card shares
+constexpr int ALONE = 48;                     // chunks up to which one workgroup finds a norm by itself: 8.0 us a call against 10.7 with a second launch; at 128 chunks 11.7 and 10.9
+// Bytes of tensors up to which a call goes through the 256 MB cache that the card shares.  Reads past it still find there what others left.
+// An update: half of the cache.  Lists in turn, the usual way / past the cache: 3 of 73 MB 20.4 / 25.2 us, 3 of 200 MB 70 / 62 us; one of 160 MB again and again 54 / 61 us, and
+// with 1 GB of other work in between 74 / 64 us.
+constexpr long long CACHE = 128ll << 20;
+// A norm by itself, 64 MB: again and again 14.7 / 15.6 us, with other work in between 30 / 18 us; 32 MB: 15.3 / 16.0 and 19 / 13 us.
+constexpr long long CACHE_NORM = 24ll << 20;
 
 struct Row { const void* p[4]; float* step; long long n; int type, type_g; long long pad; };      // BFSR_LIST_ROW bytes
 static_assert(sizeof(Row) == BFSR_LIST_ROW, "the row's size is part of the interface");
@@ -476,16 +481,15 @@ __global__ __launch_bounds__(512) void pointer_write_kernel(Pointers all, int n,
 
 bool good(const BfsrListArgs& a) { return a.rows && a.chunks && a.n > 0 && a.count >= 0 && a.count < (1 << 24) && a.chunk == CHUNK && a.bytes >= 0; }
 
-int sums_of(int count) { const int w = TN / 64, b = (count + w - 1) / w; return count <= ALONE ? 1 : b < PARTS ? b : PARTS; }
+int sums_of(int count) { const int w = TN / 64, b = (count + w - 1) / w; return b < 1 ? 1 : b < PARTS ? b : PARTS; }
 
 // Whether a call streams its tensors past the cache.
-bool streams(const BfsrListArgs& a) { return a.bytes > CACHE; }
+bool streams(const BfsrListArgs& a, long long bound) { return a.bytes > bound; }
 
 // The parts of a norm; `out`: the norm itself, which one workgroup finds. `h`: with them, the beginning of a step of Adam.
-int launch_parts(const BfsrListArgs& a, int col, bool stream, float* out, const Hyper* h, Factors* factors, hipStream_t st)
+int launch_parts(const BfsrListArgs& a, int col, bool stream, int sums, float* out, const Hyper* h, Factors* factors, hipStream_t st)
 {
     const auto k = a.max ? stream ? norm_parts_kernel<true, true> : norm_parts_kernel<true, false> : stream ? norm_parts_kernel<false, true> : norm_parts_kernel<false, false>;
-    const int sums = sums_of(a.count);
     k<<<sums + (h ? (a.n + TN - 1) / TN : 0), TN, 0, st>>>((const Row*)a.rows, (const int2*)a.chunks, (const void* const*)a.other, col, a.count, sums, (double*)a.work, out, a.n,
                                                         h ? *h : Hyper{}, factors);
     return (int)hipGetLastError();
@@ -496,6 +500,8 @@ int launch_parts(const BfsrListArgs& a, int col, bool stream, float* out, const 
 extern "C" int bfsr_list_chunk(long long total) { return total < 0 ? -1 : CHUNK; }
 
 extern "C" long long bfsr_list_work(int n) { return n < 0 ? -1 : (long long)PARTS * 8 + (long long)n * (long long)sizeof(Factors); }
+
+extern "C" long long bfsr_norm_work(int count) { return count < 0 ? -1 : count <= ALONE ? 0 : PARTS * 8; }
 
 extern "C" int bfsr_list_write(const void* const* const* cols, int ncols, const long long* sizes, const int* types, int n, int chunk, void* rows, void* chunks, void* stream)
 {
@@ -534,10 +540,11 @@ extern "C" int bfsr_pointer_write(const void* const* from, int n, void* to, void
 
 extern "C" int bfsr_grad_norm(const BfsrListArgs* a, void* stream)
 {
-    if (!a || !good(*a) || !a->work || !a->norm) return -1;
+    if (!a || !good(*a) || !a->norm || (a->count > ALONE && !a->work)) return -1;
     hipStream_t st = (hipStream_t)stream;
-    const int sums = sums_of(a->count), err = launch_parts(*a, 0, streams(*a), sums == 1 ? a->norm : nullptr, nullptr, nullptr, st);
-    if (err || sums == 1) return err;
+    if (a->count <= ALONE) return launch_parts(*a, 0, streams(*a, CACHE_NORM), 1, a->norm, nullptr, nullptr, st);
+    const int sums = sums_of(a->count), err = launch_parts(*a, 0, streams(*a, CACHE_NORM), sums, nullptr, nullptr, nullptr, st);
+    if (err) return err;
     norm_finish_kernel<<<1, 64, 0, st>>>(Norm{(const double*)a->work, sums, a->max, nullptr, a->norm, -1.f});
     return (int)hipGetLastError();
 }
@@ -546,8 +553,8 @@ extern "C" int bfsr_clip_grads(const BfsrListArgs* a, float max_norm, void* stre
 {
     if (!a || !good(*a) || !a->work || !a->norm || !(max_norm >= 0.f)) return -1;
     hipStream_t st = (hipStream_t)stream;
-    const bool past = streams(*a);
-    const int err = launch_parts(*a, 0, past, nullptr, nullptr, nullptr, st), per = T / 64;
+    const bool past = streams(*a, CACHE);
+    const int err = launch_parts(*a, 0, past, sums_of(a->count), nullptr, nullptr, nullptr, st), per = T / 64;
     if (err) return err;
     (past ? clip_kernel<true> : clip_kernel<false>)<<<a->count ? (a->count + per - 1) / per : 1, T, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, a->count,
                                                    Norm{(const double*)a->work, sums_of(a->count), a->max, nullptr, a->norm, max_norm});
@@ -563,9 +570,9 @@ extern "C" int bfsr_adam_step(const BfsrListArgs* a, const BfsrAdamArgs* h, void
     const bool norm = h->max_norm >= 0.f || h->skip_nonfinite, own = norm && !h->given_norm;
     if (norm && !a->norm) return -1;
     const Hyper hy = {h->lr, h->beta1, h->beta2, h->weight_decay, h->eps, h->decoupled, h->skip_nonfinite, h->lr_at};
-    const bool past = streams(*a);
+    const bool past = streams(*a, CACHE);
     int err;
-    if (own) err = launch_parts(*a, 1, past, nullptr, &hy, factors, st);
+    if (own) err = launch_parts(*a, 1, past, sums_of(a->count), nullptr, &hy, factors, st);
     else {
         adam_begin_kernel<<<(a->n + T - 1) / T, T, 0, st>>>((const Row*)a->rows, a->n, hy, factors);
         err = (int)hipGetLastError();

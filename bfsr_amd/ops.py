@@ -184,16 +184,18 @@ class ListTable(object):
         self.stream, self.table = None, None
         if not self.n:
             return
-        self.work = ops.lib.bfsr_list_work(self.n) // 8
+        self.norm_work = ops.lib.bfsr_norm_work(self.count) // 8
         types = np.array(types, dtype=np.int32)
         with torch.cuda.device(self.device):
             if not once and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("tensor list: make it before the capture begins (its table is written once, not at every replay)")
             stream = torch.cuda.current_stream(self.device)
             self.stream = stream.cuda_stream
-            self.table = torch.empty(self.n * 8 + max(self.count, 1), dtype=torch.int64, device=self.device)
+            # behind the table: scratch for what writes the tensors, since two such calls cannot run at the same time anyway.  A norm gets its own for each call
+            words = 8 * self.n + (self.count + 2) // 2 * 2
+            self.table = torch.empty(words + ops.lib.bfsr_list_work(self.n) // 8, dtype=torch.int64, device=self.device)
             self.rows = self.table.data_ptr()
-            self.chunks = self.rows + 64 * self.n
+            self.chunks, self.work = self.rows + 64 * self.n, self.rows + 8 * words
             cols = [np.ascontiguousarray(c) for c in cols]
             ptrs = (C.c_void_p * len(cols))(*[c.ctypes.data for c in cols])
             _lib.check(ops.lib.bfsr_list_write(ptrs, len(cols), sizes.ctypes.data, types.ctypes.data, self.n, self.chunk, self.rows, self.chunks, self.stream),
@@ -216,12 +218,14 @@ class ListTable(object):
                 self.table.record_stream(torch.cuda.current_stream(i))
             if torch.cuda.is_current_stream_capturing():
                 ops._captured_tables[id(self.table)] = self.table      # a graph reads it at every replay, whatever becomes of the list
-        other = None
+        other, work = None, self.work
         if grads is not None:
             other = torch.empty(self.n, dtype=torch.int64, device=self.device)
             _lib.check(ops.lib.bfsr_pointer_write(grads.ctypes.data, self.n, other.data_ptr(), stream), "pointer_write")
-        work = torch.empty(self.work, dtype=torch.float64, device=self.device)
-        a = _lib.BfsrListArgs(self.rows, self.chunks, self.n, self.count, self.chunk, kind, _ptr(other), self.bytes, work.data_ptr(), _ptr(norm))
+        if name == "grad_norm":
+            own = torch.empty(self.norm_work, dtype=torch.float64, device=self.device) if self.norm_work else None
+            work = _ptr(own)
+        a = _lib.BfsrListArgs(self.rows, self.chunks, self.n, self.count, self.chunk, kind, _ptr(other), self.bytes, work, _ptr(norm))
         if ops._keylog is None and ops.profile_keys is None:
             err = fn(a, *more, stream)
         else:

@@ -614,7 +614,8 @@ typedef struct BfsrListArgs {
     int max;                                 /* the norm: 0 Euclidean, 1 the largest magnitude */
     const void* other;                       /* bfsr_adam_step: NULL, or the gradients' n pointers in place of the table's (same sizes and types) */
     long long bytes;                         /* of all tensors that the call reads or writes, each once: what is larger than the cache streams past it */
-    void* work;                              /* scratch of this call alone, bfsr_list_work(n) bytes, 16-byte aligned */
+    void* work;                              /* 16-byte aligned scratch that no call shares that may run at the same time: bfsr_list_work(n) bytes, or bfsr_norm_work(count) for
+                                                bfsr_grad_norm (0: none) */
     float* norm;                             /* where the norm goes (bfsr_adam_step: only with max_norm >= 0 or skip_nonfinite) */
 } BfsrListArgs;
 typedef struct BfsrAdamArgs {
@@ -627,6 +628,7 @@ typedef struct BfsrAdamArgs {
 } BfsrAdamArgs;
 int bfsr_list_chunk(long long total);                      /* elements a chunk for a list of `total` elements */
 long long bfsr_list_work(int n);                           /* bytes of scratch */
+long long bfsr_norm_work(int count);
 int bfsr_list_write(const void* const* const* cols, int ncols, const long long* sizes, const int* types, int n, int chunk, void* rows, void* chunks, void* stream);
 int bfsr_pointer_write(const void* const* from, int n, void* to, void* stream);
 int bfsr_grad_norm(const BfsrListArgs* a, void* stream);

@@ -103,10 +103,11 @@ def test_c_entries_refuse_before_a_launch():
     assert lib.bfsr_pointer_write(None, 1, 4096, None) == lib.bfsr_pointer_write(one, 0, 4096, None) == lib.bfsr_pointer_write(one, 1, None, None) == -1
     a, h = _lib.BfsrListArgs(), _lib.BfsrAdamArgs()
     good = dict(rows=4096, chunks=4096, n=1, count=1, chunk=chunk, work=4096, norm=4096)
-    for bad in (dict(rows=None), dict(chunks=None), dict(n=0), dict(count=-1), dict(count=1 << 24), dict(chunk=0), dict(chunk=1000), dict(work=None), dict(norm=None)):
+    for bad in (dict(rows=None), dict(chunks=None), dict(n=0), dict(count=-1), dict(count=1 << 24), dict(chunk=0), dict(chunk=1000), dict(work=None, count=1000), dict(norm=None)):
         for k, v in dict(good, **bad).items():
             setattr(a, k, v)
         h.beta1, h.beta2, h.max_norm = 0.9, 0.999, 1.0
+        assert lib.bfsr_norm_work(1000) > 0 == lib.bfsr_norm_work(1) and lib.bfsr_norm_work(-1) == -1
         assert lib.bfsr_grad_norm(C.byref(a), None) == lib.bfsr_clip_grads(C.byref(a), 1.0, None) == lib.bfsr_adam_step(C.byref(a), C.byref(h), None) == -1, bad
     for k, v in good.items():
         setattr(a, k, v)
