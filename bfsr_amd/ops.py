@@ -210,10 +210,7 @@ class ListTable(object):
             with torch.cuda.device(i):
                 return self.call(name, fn, kind, norm, *more, grads=grads)
         ops, stream = self.ops, torch._C._cuda_getCurrentRawStream(i)
-        if self.once:
-            if stream != self.stream:
-                raise RuntimeError("tensor list: one made with once=True belongs to the stream it was made on")
-        else:
+        if not self.once:
             if stream != self.stream:
                 self.table.record_stream(torch.cuda.current_stream(i))
             if torch.cuda.is_current_stream_capturing():
@@ -264,6 +261,8 @@ class TensorList(ListTable):
     """A list of tensors for grad_norm and clip_grads (HipOps.tensor_list)."""
 
     def __init__(self, ops, tensors, out=None, once=False):
+        """`once`: for one call that follows at once on the same stream; made without waiting, and also while a graph is captured, which then writes the table at every
+        replay.  Such a list is never handed out: kept, it could be read where its table has not been written."""
         dev = ops._index_device()
         tensors = list_column(tensors, dev, "tensor_list", alias=False)
         at, nbytes = _addresses(tensors), _bytes(tensors)
@@ -448,35 +447,44 @@ class HipOps(object):
         return d if d.index is not None else torch.device(d.type, torch.cuda.current_device())
 
     # ---- lists of tensors: the end of a training step ------------------------------------------
-    def tensor_list(self, tensors, out=None, once=False):
+    def tensor_list(self, tensors, out=None):
         """A handle of a list of gradients for grad_norm and clip_grads: dense float32 / float16 / bfloat16 tensors on this device, in any mixture, order of
         axes and alignment, empty ones among them.  `out`: tensors of the same shapes, orders and types that take the clipped values (default: in place).
 
-        The handle stands for the memory that the tensors have now: their values are read at each call, but a gradient that is made anew (zero_grad with
-        set_to_none) needs a new handle.  Making one waits for the current stream; it may then be used on any stream, and in graphs, which have to be
-        captured after it was made.  once=True: a handle for the current stream alone, made without waiting, also while a graph is captured."""
-        return TensorList(self, tensors, out, once)
+        The handle stands for the memory that the tensors have now, and holds it: their values are read at each call, but a gradient that is made anew (zero_grad
+        with set_to_none) needs a new handle, and so does one whose storage is resized.  Making one waits for the current stream; it may then be used on any
+        stream, and in graphs, which have to be captured after it was made.  Two calls that write the same tensors cannot run at the same time; norms can."""
+        return TensorList(self, tensors, out)
 
     def grad_norm(self, tensors, norm_type=2.0, out=None):
-        """The norm of all elements of a tensor_list: 2 (summed in 64 bits, so finite gradients have a finite norm as far as float32 holds it) or inf.
-        NaN where an element is.  Returns a 0-d float32 on the device (`out`, if given)."""
-        kind, norm = _norm_type(norm_type), self._norm_out(tensors, out)
+        """The norm of all elements of a tensor_list, or of a plain list of tensors (whose table is then made for this one call, without waiting): 2 (summed in
+        64 bits, so finite gradients have a finite norm as far as float32 holds it) or inf.  NaN where an element is.
+        Returns a 0-d float32 on the device (`out`, if given)."""
+        kind, tensors = _norm_type(norm_type), self._listed(tensors)
+        norm = self._norm_out(tensors, out)
         if tensors.n:
             tensors.call("grad_norm", self.lib.bfsr_grad_norm, kind, norm)
         return norm
 
     def clip_grads(self, tensors, max_norm, norm_type=2.0):
-        """Multiplies a tensor_list by min(1, max_norm / (norm + 1e-6)), in place or into its `out`; returns the norm before (0-d float32, on the device).
-        An infinite norm makes finite gradients 0, a NaN makes all NaN, as the quotient does.  Products are rounded once, to the tensor's type."""
-        kind, max_norm, norm = _norm_type(norm_type), _at_least_0(max_norm, "clip_grads.max_norm"), self._norm_out(tensors, None)
+        """Multiplies a tensor_list, in place or into its `out`, or a plain list of tensors in place, by min(1, max_norm / (norm + 1e-6)); returns the norm
+        before (0-d float32, on the device).  An infinite norm makes finite gradients 0, a NaN makes all NaN, as the quotient does.  Products are rounded
+        once, to the tensor's type."""
+        kind, max_norm, tensors = _norm_type(norm_type), _at_least_0(max_norm, "clip_grads.max_norm"), self._listed(tensors)
+        norm = self._norm_out(tensors, None)
         if tensors.n:
             tensors.call("clip_grads", self.lib.bfsr_clip_grads, kind, norm, max_norm)
             torch.autograd.graph.increment_version(tensors.written)
         return norm
 
+    def _listed(self, tensors):
+        if not isinstance(tensors, TensorList):
+            return TensorList(self, tensors, None, once=True)
+        if tensors.ops is not self:
+            raise ValueError("tensor list: it belongs to another ops object")
+        return tensors
+
     def _norm_out(self, tensors, out):
-        if not isinstance(tensors, TensorList) or tensors.ops is not self:
-            raise TypeError("need a handle from this object's tensor_list()")
         dev = tensors.device
         if out is not None:
             _one_float(out, dev, "grad_norm.out")
@@ -486,7 +494,8 @@ class HipOps(object):
     def adam(self, params, grads, exp_avg, exp_avg_sq, step):
         """A plan of Adam's update of `params` (float32 / float16 / bfloat16; gradients of any of these, moments float32, all in the parameter's shape and
         order of axes).  grads=None: every run() brings its own, of the parameters' types, and the plan holds none.  step: the counts of steps taken, a 1-d float32 tensor or a list of tensors of one float32.  AdamPlan.run() makes a step.
-        Like a tensor_list, the plan stands for the memory that the tensors have now, and making it waits for the current stream."""
+        Like a tensor_list, the plan stands for the memory that the tensors have now, and making it waits for the current stream.  Steps of one plan cannot run
+        at the same time."""
         return AdamPlan(self, params, grads, exp_avg, exp_avg_sq, step)
 
     # ---- conv -----------------------------------------------------------------------------

@@ -32,7 +32,7 @@ def clip_grad_norm(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False
     if not grads:
         return torch.zeros(())
     ops = ops or _ops_of(grads[0])
-    norm = ops.clip_grads(ops.tensor_list(grads, once=True), max_norm, norm_type)
+    norm = ops.clip_grads(grads, max_norm, norm_type)
     if error_if_nonfinite and not torch.isfinite(norm):
         raise RuntimeError("bfsr_amd.optim.clip_grad_norm: the norm of the gradients is %r" % float(norm))
     return norm
@@ -87,6 +87,8 @@ class Adam(torch.optim.Optimizer):
     def _state_of(self, params):
         new = [p for p in params if not self.state[p]]
         if new:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("Adam: take an ordinary step before the capture begins (it makes the state)")
             for p, step in zip(new, torch.zeros(len(new), dtype=torch.float32, device=new[0].device).unbind()):
                 self.state[p] = {"step": step, "exp_avg": self._moment(p), "exp_avg_sq": self._moment(p)}
         return [self.state[p] for p in params]
@@ -134,7 +136,7 @@ class Adam(torch.optim.Optimizer):
         norm = None
         if wants and len(work) > 1:
             ops = work[0][1].ops
-            norm = ops.grad_norm(ops.tensor_list([g for w in work for g in w[2]], once=True))
+            norm = ops.grad_norm([g for w in work for g in w[2]])
         for group, plan, _, found in work:
             lr = group["lr"]
             if isinstance(lr, torch.Tensor) and lr.device.type == "cpu":

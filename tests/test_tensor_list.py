@@ -162,10 +162,8 @@ def test_train_step_clips_with_the_models_ops(golden_dir):
     import bfsr_amd.linf.train as train
 
     class Double(CpuOps):
-        def tensor_list(self, tensors, out=None, once=False):
-            return O.list_column(tensors, CPU, "x")
-
         def clip_grads(self, tensors, max_norm, norm_type=2.0):
+            tensors = O.list_column(tensors, CPU, "x")
             norm = torch.sqrt(sum(t.double().square().sum() for t in tensors)).float()
             for t in tensors:
                 t.mul_((max_norm / (norm + 1e-6)).clamp(max=1.0))
@@ -303,7 +301,7 @@ def test_orders_of_axes(hip):
 @pytest.mark.parametrize("kind", [2.0, math.inf])
 def test_far_and_near_magnitudes(hip, kind):
     """Squares that overflow or vanish in 32 bits."""
-    for scale in (1e30, 1e-30):
+    for scale in (1e30, 1e-30, 1e-40):
         ts = make(5, scale=scale)
         want = doubles(ts)
         norm = norm64(want, kind)
@@ -355,6 +353,34 @@ def test_offsets_beyond_32_bits(hip):
 
 
 @gpu
+@pytest.mark.parametrize("types", TYPES)
+def test_plain_lists(hip, types):
+    """A list of tensors in place of a handle, on any stream."""
+    ts = make(9, types=types)
+    want = doubles(ts)
+    near_norm(hip.grad_norm(ts), norm64(want))
+    near_norm(hip.grad_norm(iter(ts), math.inf), norm64(want, math.inf))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        norm = hip.clip_grads(ts, 1.0)
+    torch.cuda.synchronize()
+    near_norm(norm, norm64(want))
+    near_clipped(ts, want, min(1.0, 1.0 / (norm64(want) + 1e-6)))
+    assert float(hip.grad_norm([])) == 0.0
+
+
+@gpu
+@pytest.mark.parametrize("most", [0.0, math.inf])
+def test_extreme_bounds(hip, most):
+    ts = make(10, types=(F32, BF16))
+    want = doubles(ts)
+    hip.clip_grads(ts, most)
+    near_clipped(ts, want, 0.0 if most == 0.0 else 1.0)
+    zeros = [torch.zeros(5, device="cuda:0")]
+    assert float(hip.clip_grads(zeros, most)) == 0.0 and not bool(zeros[0].any())
+
+
+@gpu
 def test_same_bits_every_time(hip):
     ts = make(7, shapes=[(100003,), (512, 300), (7,)] * 20, types=(F32, BF16))
     tl = hip.tensor_list(ts)
@@ -372,17 +398,16 @@ def test_lists_are_refused(hip):
         with pytest.raises(ValueError):
             hip.tensor_list([a, b], out=out)
     tl = hip.tensor_list([a])
-    with pytest.raises(TypeError):
-        hip.grad_norm([a])
-    with pytest.raises(TypeError):
+    for bad, error in ((a, TypeError), ([a, 1.0], TypeError), ([a, a], ValueError)):
+        for call in (hip.grad_norm, lambda t: hip.clip_grads(t, 1.0), hip.tensor_list):
+            with pytest.raises(error):
+                call(bad)
+    with pytest.raises(ValueError):
         O.HipOps("cuda:0").grad_norm(tl)
     for call in (lambda: hip.grad_norm(tl, 1.0), lambda: hip.clip_grads(tl, -1.0), lambda: hip.clip_grads(tl, math.nan), lambda: hip.grad_norm(tl, out=torch.zeros(2, device="cuda:0")),
                  lambda: hip.grad_norm(tl, out=torch.zeros(1))):
         with pytest.raises(ValueError):
             call()
-    once = hip.tensor_list([a], once=True)
-    with torch.cuda.stream(torch.cuda.Stream()), pytest.raises(RuntimeError):
-        hip.grad_norm(once)
     empty = hip.tensor_list([])
     assert float(hip.grad_norm(empty)) == 0.0 == float(hip.clip_grads(empty, 1.0)) and float(hip.grad_norm(empty, out=torch.ones((), device="cuda:0"))) == 0.0
 
@@ -723,6 +748,10 @@ def test_captured_training_step(hip):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         steps(net, opts[1], 1, x)
+        fresh = optim.Adam(net.parameters(), ops=hip)
+        with pytest.raises(RuntimeError):
+            fresh.step()                                                    # would make its state at every replay
+        assert not any(fresh.state[p] for p in net.parameters())
     steps(eager, opts[0], 2, x)
     for k in range(4):
         lr.fill_(0.01 / (k + 1))
