@@ -20,6 +20,11 @@ constexpr int TN = 1024;                      // threads of one that sums
 constexpr int CHUNK = 2048;                   // elements of a chunk
 constexpr int PARTS = 256;                    // partial results of a norm at most, one for each of its workgroups: one a CU, and four a lane for the wave that joins them
 constexpr int ALONE = 48;                     // chunks up to which one workgroup finds a norm by itself: 8.0 us a call against 10.7 with a second launch; at 128 chunks 11.7 and 10.9
+// ... and up to which (and bytes of tensors) it clips a list, or takes a step, in the same launch.  One workgroup / a launch for each part, us a call among others and (waited for):
+// clipping 24 full chunks 7.6 (22.0) / 10.2 (21.0), 42 chunks of 0.5 MB 9.9 (24.1) / 10.6 (21.4);  a step of 11 chunks of 118 KB 6.6 (20.1) / 9.7 (20.5), clipped
+// 8.5 (23.6) / 11.7 (22.4), of 12 full chunks 10.2 (24.0) / 9.4 (20.2).  Above, one CU's share of the bandwidth counts for more than a launch.
+constexpr int ALONE_CLIP = 32, ALONE_CLIP_BYTES = 384 << 10, ALONE_ADAM = 12, ALONE_ADAM_BYTES = 192 << 10;
+constexpr int ALONE_ROWS = 256;               // rows that such a step has room for
 // Bytes of tensors up to which a call goes through the 256 MB cache that the card shares.  Reads past it still find there what others left.
 // An update: half of the cache.  Lists in turn, the usual way / past the cache: 3 of 73 MB 20.4 / 25.2 us, 3 of 200 MB 70 / 62 us; one of 160 MB again and again 54 / 61 us, and
 // with 1 GB of other work in between 74 / 64 us.
@@ -241,22 +246,16 @@ __global__ __launch_bounds__(T) void adam_begin_kernel(const Row* __restrict__ r
     if (k < n) begin_row(rows[k], h, factors + k);
 }
 
-// One part of the norm for each of the first `sums` workgroups (with one, the norm itself); those behind them, if any, begin a step of Adam.
+// The part of workgroup `index` of `of` of them (of TN threads), for every thread of it.  All its reads have been made when it is known.
 template <bool MAX, bool STREAM>
-__global__ __launch_bounds__(TN) void norm_parts_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other,
-                                                        int col, int count, int sums, double* __restrict__ parts, float* __restrict__ out, int n, Hyper h,
-                                                        Factors* __restrict__ factors)
+__device__ __forceinline__ double sum_chunks(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other, int col, int count,
+                                             int index, int of)
 {
-    if ((int)blockIdx.x >= sums) {
-        const int k = ((int)blockIdx.x - sums) * TN + threadIdx.x;
-        if (k < n) begin_row(rows[k], h, factors + k);
-        return;
-    }
     constexpr int WAVES = TN / 64;
     __shared__ double part[WAVES];
     Acc<MAX> acc;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int c = blockIdx.x * WAVES + wave; c < count; c += sums * WAVES) {
+    for (int c = index * WAVES + wave; c < count; c += of * WAVES) {
         const int2 at = chunks[c];
         const Row& r = rows[at.x];
         const void* p = other ? other[at.x] : r.p[col];
@@ -270,12 +269,24 @@ __global__ __launch_bounds__(TN) void norm_parts_kernel(const Row* __restrict__ 
     const double mine = wave_join<MAX>(acc.part());
     if ((threadIdx.x & 63) == 0) part[wave] = mine;
     __syncthreads();
-    if (threadIdx.x < 64) {
-        const double all = wave_join<MAX>(threadIdx.x < WAVES ? part[threadIdx.x] : 0.0);
-        if (threadIdx.x == 0) {
-            if (out) *out = (float)Acc<MAX>::whole(all);
-            else parts[blockIdx.x] = all;
-        }
+    return wave_join<MAX>((threadIdx.x & 63) < WAVES ? part[threadIdx.x & 63] : 0.0);
+}
+
+// One part of the norm for each of the first `sums` workgroups (with one, the norm itself); those behind them, if any, begin a step of Adam.
+template <bool MAX, bool STREAM>
+__global__ __launch_bounds__(TN) void norm_parts_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other,
+                                                        int col, int count, int sums, double* __restrict__ parts, float* __restrict__ out, int n, Hyper h,
+                                                        Factors* __restrict__ factors)
+{
+    if ((int)blockIdx.x >= sums) {
+        const int k = ((int)blockIdx.x - sums) * TN + threadIdx.x;
+        if (k < n) begin_row(rows[k], h, factors + k);
+        return;
+    }
+    const double all = sum_chunks<MAX, STREAM>(rows, chunks, other, col, count, blockIdx.x, sums);
+    if (threadIdx.x == 0) {
+        if (out) *out = (float)Acc<MAX>::whole(all);
+        else parts[blockIdx.x] = all;
     }
 }
 
@@ -285,8 +296,8 @@ __global__ __launch_bounds__(64) void norm_finish_kernel(Norm f)
     if (threadIdx.x == 0) *f.out = (float)norm;
 }
 
-template <bool STREAM, int TYPE, bool FULL>
-__device__ __forceinline__ void clip_chunk(const Norm& f, const void* from, void* to, int count)
+template <bool STREAM, int TYPE, bool FULL, class SHARE>
+__device__ __forceinline__ void clip_chunk(const SHARE& share, const void* from, void* to, int count)
 {
     typedef typename Vec<TYPE>::type V;
     constexpr int N = Vec<TYPE>::N, U = CHUNK / (64 * N);
@@ -303,9 +314,7 @@ __device__ __forceinline__ void clip_chunk(const Norm& f, const void* from, void
     const int last = count / N * N + lane;
     typename Vec<TYPE>::one e = {};
     if (more) e = p[last];
-    const double norm = whole(f);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *f.out = (float)norm;
-    const float s = share_of(f, norm);
+    const float s = share();                                       // with the loads under way
     if (s == 1.f && from == to) return;                            // in place, and nothing to change
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -317,29 +326,45 @@ __device__ __forceinline__ void clip_chunk(const Norm& f, const void* from, void
     if (more) q[last] = Vec<TYPE>::narrow(Vec<TYPE>::wide(e) * s);
 }
 
-// One chunk for each wave, and then the wave ends: one that went on to another chunk would wait for its stores before the next loads count as arrived.
-// Chunks are taken from the end, where the cache holds what the norm has read last.
-template <bool STREAM>
-__global__ __launch_bounds__(T) void clip_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, int count, Norm f)
+template <bool STREAM, class SHARE>
+__device__ __forceinline__ void clip_one(const Row* __restrict__ rows, const int2 at, const SHARE& share)
 {
-    const int c = count - 1 - (int)blockIdx.x * (T / 64) - __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (c < 0) {
-        if (count == 0 && threadIdx.x == 0) *f.out = (float)whole(f);
-        return;
-    }
-    const int2 at = chunks[c];
     const Row& r = rows[at.x];
     const long long begin = (long long)at.y * CHUNK;
     const int left = left_in(r, begin);
     const void* from = at_element(r.p[0], r.type, begin);
     void* to = at_element(r.p[1], r.type, begin);
     const bool full = left == CHUNK;
-    if (r.type == BFSR_LIST_F32) full ? clip_chunk<STREAM, BFSR_LIST_F32, true>(f, from, to, left) : clip_chunk<STREAM, BFSR_LIST_F32, false>(f, from, to, left);
-    else if (r.type == BFSR_LIST_F16) full ? clip_chunk<STREAM, BFSR_LIST_F16, true>(f, from, to, left) : clip_chunk<STREAM, BFSR_LIST_F16, false>(f, from, to, left);
-    else full ? clip_chunk<STREAM, BFSR_LIST_BF16, true>(f, from, to, left) : clip_chunk<STREAM, BFSR_LIST_BF16, false>(f, from, to, left);
+    if (r.type == BFSR_LIST_F32) full ? clip_chunk<STREAM, BFSR_LIST_F32, true>(share, from, to, left) : clip_chunk<STREAM, BFSR_LIST_F32, false>(share, from, to, left);
+    else if (r.type == BFSR_LIST_F16) full ? clip_chunk<STREAM, BFSR_LIST_F16, true>(share, from, to, left) : clip_chunk<STREAM, BFSR_LIST_F16, false>(share, from, to, left);
+    else full ? clip_chunk<STREAM, BFSR_LIST_BF16, true>(share, from, to, left) : clip_chunk<STREAM, BFSR_LIST_BF16, false>(share, from, to, left);
 }
 
-struct Rule { float b1, c1, b2, c2, wd, eps; bool add, keep, skip; Factors f; };
+// One chunk for each wave, and then the wave ends: one that went on to another chunk would wait for its stores before the next loads count as arrived.
+// Chunks are taken from the end, where the cache holds what the norm has read last.
+template <bool STREAM>
+__global__ __launch_bounds__(T) void clip_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, int count, Norm f)
+{
+    const int c = count - 1 - (int)blockIdx.x * (T / 64) - __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (c < 0) return;
+    clip_one<STREAM>(rows, chunks[c], [&] {
+        const double norm = whole(f);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *f.out = (float)norm;
+        return share_of(f, norm);
+    });
+}
+
+// A short list in one workgroup: the norm, and then the clipping of what its caches still hold.
+template <bool MAX>
+__global__ __launch_bounds__(TN) void clip_alone_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, int count, Norm f)
+{
+    const double norm = Acc<MAX>::whole(sum_chunks<MAX, false>(rows, chunks, nullptr, 0, count, 0, 1));
+    if (threadIdx.x == 0) *f.out = (float)norm;
+    const float s = share_of(f, norm);
+    for (int c = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); c < count; c += TN / 64) clip_one<false>(rows, chunks[c], [=] { return s; });
+}
+
+struct Rule { float b1, c1, b2, c2, wd, eps; bool add, keep; Factors f; };
 
 __device__ __forceinline__ void adam_element(const Rule& w, float share, float& p, float g, float& m, float& v)
 {
@@ -351,14 +376,16 @@ __device__ __forceinline__ void adam_element(const Rule& w, float share, float& 
     p -= w.f.size * (m / fmaf(sqrtf(v), w.f.root, w.eps));
 }
 
-template <bool STREAM>
-__device__ __forceinline__ void adam_chunk(const Norm& f, void* pp, const void* gp, float* mp, float* vp, int type, int type_g, int count, const Rule& w)
+// One chunk for T threads; `share`: what its gradients are multiplied by, below 0 where the step is skipped.
+template <bool STREAM, class SHARE>
+__device__ __forceinline__ void adam_chunk(const SHARE& share_of_step, void* pp, const void* gp, float* mp, float* vp, int type, int type_g, int count, const Rule& w)
 {
     constexpr int U = CHUNK / (T * 4), F32 = BFSR_LIST_F32;
+    const int t = threadIdx.x & (T - 1);
     Four p[U], g[U], m[U], v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int i = (u * T + threadIdx.x) * 4;
+        const int i = (u * T + t) * 4;
         if (i + 4 <= count) {
             p[u] = load4<STREAM>(pp, type, i);
             g[u] = load4<STREAM>(gp, type_g, i);
@@ -366,15 +393,11 @@ __device__ __forceinline__ void adam_chunk(const Norm& f, void* pp, const void* 
             v[u] = load4<STREAM>(vp, F32, i);
         }
     }
-    float share = 1.f;
-    if (f.out) {
-        const double norm = whole(f);
-        if (w.skip && !(norm <= 1.7976931348623157e308)) return;
-        share = share_of(f, norm);
-    }
+    const float share = share_of_step();                           // with the loads under way
+    if (share < 0.f) return;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int i = (u * T + threadIdx.x) * 4;
+        const int i = (u * T + t) * 4;
         if (i + 4 <= count) {
             f4 x = floats(p[u], type), y = floats(g[u], type_g), m1 = m[u].f, v1 = v[u].f;
 #pragma unroll
@@ -388,8 +411,8 @@ __device__ __forceinline__ void adam_chunk(const Norm& f, void* pp, const void* 
             store4<STREAM>(vp, F32, i, v1);
         }
     }
-    if ((int)threadIdx.x < (count & 3)) {                          // what does not fill a load
-        const int i = (count & ~3) + threadIdx.x;
+    if (t < (count & 3)) {                          // what does not fill a load
+        const int i = (count & ~3) + t;
         float a = load1(pp, type, i), b = mp[i], c = vp[i];
         adam_element(w, share, a, load1(gp, type_g, i), b, c);
         store1(pp, type, i, a);
@@ -397,6 +420,24 @@ __device__ __forceinline__ void adam_chunk(const Norm& f, void* pp, const void* 
         vp[i] = c;
     }
 }
+
+template <bool STREAM, class SHARE>
+__device__ __forceinline__ void adam_one(const Row* __restrict__ rows, const int2 at, const void* const* __restrict__ other, const Hyper& h, const Factors& factors,
+                                         const SHARE& share)
+{
+    Rule w = {(float)h.beta1, (float)(1.0 - h.beta1), (float)h.beta2, (float)(1.0 - h.beta2), (float)h.weight_decay, h.eps};
+    w.add = w.wd != 0.f && !h.decoupled;
+    w.keep = w.wd != 0.f && h.decoupled;
+    w.f = factors;
+    const Row& r = rows[at.x];
+    const long long begin = (long long)at.y * CHUNK;
+    void* p = at_element(r.p[0], r.type, begin);
+    const void* g = at_element(other ? other[at.x] : r.p[1], r.type_g, begin);
+    adam_chunk<STREAM>(share, p, g, (float*)r.p[2] + begin, (float*)r.p[3] + begin, r.type, r.type_g, left_in(r, begin), w);
+}
+
+// The share of a step, or -1 where it is skipped: its norm is infinite or NaN, and the caller asked for that.
+__device__ __forceinline__ float share_of_step(const Norm& f, const Hyper& h, double norm) { return h.skip && !(norm <= 1.7976931348623157e308) ? -1.f : share_of(f, norm); }
 
 // One chunk for each workgroup; the last workgroup sees to the norm's output, and to the counts of a step that is skipped.
 template <bool STREAM>
@@ -408,23 +449,37 @@ __global__ __launch_bounds__(T) void adam_kernel(const Row* __restrict__ rows, c
         if (!f.out) return;
         const double norm = whole(f);
         if (threadIdx.x == 0) *f.out = (float)norm;
-        if (h.skip && !(norm <= 1.7976931348623157e308))           // infinite or NaN
+        if (share_of_step(f, h, norm) < 0.f)
             for (int k = threadIdx.x; k < n; k += T) *rows[k].step = factors[k].had;
         return;
     }
-    Rule w = {(float)h.beta1, (float)(1.0 - h.beta1), (float)h.beta2, (float)(1.0 - h.beta2), (float)h.weight_decay, h.eps};
-    w.add = w.wd != 0.f && !h.decoupled;
-    w.keep = w.wd != 0.f && h.decoupled;
-    w.skip = h.skip;
     const int2 at = chunks[c];
-    const Row& r = rows[at.x];
-    w.f = factors[at.x];
-    const long long begin = (long long)at.y * CHUNK;
-    void* p = at_element(r.p[0], r.type, begin);
-    const void* g = at_element(other ? other[at.x] : r.p[1], r.type_g, begin);
-    float* m = (float*)r.p[2] + begin;
-    float* v = (float*)r.p[3] + begin;
-    adam_chunk<STREAM>(f, p, g, m, v, r.type, r.type_g, left_in(r, begin), w);
+    adam_one<STREAM>(rows, at, other, h, factors[at.x], [&] { return f.out ? share_of_step(f, h, whole(f)) : 1.f; });
+}
+
+// A short list in one workgroup: the counts, the norm if there is to be one, and the update of what its caches still hold.
+template <bool MAX>
+__global__ __launch_bounds__(TN) void adam_alone_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other, int count, int n,
+                                                        Norm f, Hyper h)
+{
+    __shared__ Factors factors[ALONE_ROWS];
+    const int k = threadIdx.x;
+    if (k < n) begin_row(rows[k], h, factors + k);
+    float share = 1.f;
+    if (f.out) {
+        const double norm = f.given ? (double)*f.given : Acc<MAX>::whole(sum_chunks<MAX, false>(rows, chunks, other, 1, count, 0, 1));
+        if (k == 0) *f.out = (float)norm;
+        share = share_of_step(f, h, norm);
+        if (share < 0.f) {
+            if (k < n) *rows[k].step = factors[k].had;
+            return;
+        }
+    }
+    __syncthreads();
+    for (int c = __builtin_amdgcn_readfirstlane(k / T); c < count; c += TN / T) {
+        const int2 at = chunks[c];
+        adam_one<false>(rows, at, other, h, factors[at.x], [=] { return share; });
+    }
 }
 
 // ---- the table: rows and chunks travel to the device as kernel arguments.  No host buffer has to outlive the call, nothing waits for the stream, and a
@@ -542,7 +597,7 @@ extern "C" int bfsr_grad_norm(const BfsrListArgs* a, void* stream)
 {
     if (!a || !good(*a) || !a->norm || (a->count > ALONE && !a->work)) return -1;
     hipStream_t st = (hipStream_t)stream;
-    if (a->count <= ALONE) return launch_parts(*a, 0, streams(*a, CACHE_NORM), 1, a->norm, nullptr, nullptr, st);
+    if (a->count <= ALONE) return launch_parts(*a, 0, false, 1, a->norm, nullptr, nullptr, st);
     const int sums = sums_of(a->count), err = launch_parts(*a, 0, streams(*a, CACHE_NORM), sums, nullptr, nullptr, nullptr, st);
     if (err) return err;
     norm_finish_kernel<<<1, 64, 0, st>>>(Norm{(const double*)a->work, sums, a->max, nullptr, a->norm, -1.f});
@@ -553,10 +608,15 @@ extern "C" int bfsr_clip_grads(const BfsrListArgs* a, float max_norm, void* stre
 {
     if (!a || !good(*a) || !a->work || !a->norm || !(max_norm >= 0.f)) return -1;
     hipStream_t st = (hipStream_t)stream;
+    const Norm one = {nullptr, 0, a->max, nullptr, a->norm, max_norm};
+    if (!a->count || (a->count <= ALONE_CLIP && a->bytes <= ALONE_CLIP_BYTES)) {
+        (a->max ? clip_alone_kernel<true> : clip_alone_kernel<false>)<<<1, TN, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, a->count, one);
+        return (int)hipGetLastError();
+    }
     const bool past = streams(*a, CACHE);
     const int err = launch_parts(*a, 0, past, sums_of(a->count), nullptr, nullptr, nullptr, st), per = T / 64;
     if (err) return err;
-    (past ? clip_kernel<true> : clip_kernel<false>)<<<a->count ? (a->count + per - 1) / per : 1, T, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, a->count,
+    (past ? clip_kernel<true> : clip_kernel<false>)<<<(a->count + per - 1) / per, T, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, a->count,
                                                    Norm{(const double*)a->work, sums_of(a->count), a->max, nullptr, a->norm, max_norm});
     return (int)hipGetLastError();
 }
@@ -570,6 +630,13 @@ extern "C" int bfsr_adam_step(const BfsrListArgs* a, const BfsrAdamArgs* h, void
     const bool norm = h->max_norm >= 0.f || h->skip_nonfinite, own = norm && !h->given_norm;
     if (norm && !a->norm) return -1;
     const Hyper hy = {h->lr, h->beta1, h->beta2, h->weight_decay, h->eps, h->decoupled, h->skip_nonfinite, h->lr_at};
+    const float* given = norm ? h->given_norm : nullptr;
+    const float max_norm = h->max_norm >= 0.f ? h->max_norm : -1.f;
+    if (a->count <= ALONE_ADAM && a->bytes <= ALONE_ADAM_BYTES && a->n <= ALONE_ROWS) {
+        (a->max ? adam_alone_kernel<true> : adam_alone_kernel<false>)<<<1, TN, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, (const void* const*)a->other, a->count, a->n,
+                                                                                       Norm{nullptr, 0, a->max, given, norm ? a->norm : nullptr, max_norm}, hy);
+        return (int)hipGetLastError();
+    }
     const bool past = streams(*a, CACHE);
     int err;
     if (own) err = launch_parts(*a, 1, past, sums_of(a->count), nullptr, &hy, factors, st);
@@ -579,7 +646,6 @@ extern "C" int bfsr_adam_step(const BfsrListArgs* a, const BfsrAdamArgs* h, void
     }
     if (err) return err;
     (past ? adam_kernel<true> : adam_kernel<false>)<<<a->count + 1, T, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, (const void* const*)a->other, a->count, a->n,
-                                                   Norm{(const double*)a->work, own ? sums_of(a->count) : 0, a->max, norm ? h->given_norm : nullptr, norm ? a->norm : nullptr,
-                                                        h->max_norm >= 0.f ? h->max_norm : -1.f}, hy, factors);
+                                                   Norm{(const double*)a->work, own ? sums_of(a->count) : 0, a->max, given, norm ? a->norm : nullptr, max_norm}, hy, factors);
     return (int)hipGetLastError();
 }

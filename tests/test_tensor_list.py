@@ -203,6 +203,10 @@ def hip():
 SIZES = [(1,), (2,), (3,), (0,), (4,), (5, 1), (63,), (64,), (), (1023,), (1024,), (1025,), (4095,), (64, 64), (4097,), (16, 9, 3, 3), (37, 37, 3, 3), (12289,)]
 
 
+SHORT = [(1,), (0,), (5, 1), (63,), (), (1025,), (2048,), (2051,)]          # one workgroup clips it, and takes a step, by itself
+LONG = SIZES + [(300001,)]                                                  # ... and several
+
+
 def make(seed, shapes=SIZES, types=(F32,), scale=1.0, lead=0):
     """Tensors on the GPU, the types in turn; `lead` > 0: views that start `lead` elements into a buffer (no alignment but the element's)."""
     g = torch.Generator().manual_seed(seed)
@@ -272,8 +276,9 @@ def test_norm_and_clip_of_many_and_few(hip, shapes):
 @pytest.mark.parametrize("lead", [0, 1])
 @pytest.mark.parametrize("types", TYPES)
 @pytest.mark.parametrize("kind", [2.0, math.inf])
-def test_clip_in_place(hip, types, kind, lead):
-    ts = make(3, types=types, lead=lead, scale=0.5)
+@pytest.mark.parametrize("shapes", [SHORT, LONG])
+def test_clip_in_place(hip, shapes, types, kind, lead):
+    ts = make(3, shapes, types=types, lead=lead, scale=0.5)
     want, versions = doubles(ts), [t._version for t in ts]
     norm = norm64(want, kind)
     near_norm(hip.clip_grads(hip.tensor_list(ts), 0.25 * norm, kind), norm)
@@ -314,8 +319,9 @@ def test_far_and_near_magnitudes(hip, kind):
 @pytest.mark.parametrize("kind", [2.0, math.inf])
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
 @pytest.mark.parametrize("at", [0, 7, 16])
-def test_not_finite(hip, kind, bad, at):
-    ts = make(6, types=(F32, BF16, F16))
+@pytest.mark.parametrize("shapes", [SIZES, LONG])
+def test_not_finite(hip, shapes, kind, bad, at):
+    ts = make(6, shapes, types=(F32, BF16, F16))
     ts[at].reshape(-1)[-1] = bad
     norm = hip.grad_norm(hip.tensor_list(ts), kind)
     assert math.isnan(float(norm)) if math.isnan(bad) else float(norm) == math.inf
@@ -367,6 +373,8 @@ def test_plain_lists(hip, types):
     near_norm(norm, norm64(want))
     near_clipped(ts, want, min(1.0, 1.0 / (norm64(want) + 1e-6)))
     assert float(hip.grad_norm([])) == 0.0
+    empty = [torch.zeros(0, device="cuda:0")] * 2
+    assert float(hip.grad_norm(empty)) == 0.0 == float(hip.clip_grads(hip.tensor_list(empty), 1.0, math.inf))
 
 
 @gpu
@@ -478,8 +486,9 @@ def check_adam(hip, p, g, m, v, step, plan=None, share=1.0, norm=None, lr=1e-2, 
 @gpu
 @pytest.mark.parametrize("lead", [0, 1])
 @pytest.mark.parametrize("types, grad_types", [((F32,), (F32,)), ((BF16,), (BF16,)), ((F16,), (F16,)), ((F32,), (BF16,)), ((F32,), (F16,)), ((F32, BF16, F16), (F16, F32, BF16, BF16))])
-def test_adam_types(hip, types, grad_types, lead):
-    case = adam_case(20, SIZES, types, grad_types, lead)
+@pytest.mark.parametrize("shapes", [SHORT, SIZES])
+def test_adam_types(hip, shapes, types, grad_types, lead):
+    case = adam_case(20, shapes, types, grad_types, lead)
     plan = check_adam(hip, *case)
     check_adam(hip, *case, plan=plan, wd=0.1)
     for c in (case[0], case[2]):
@@ -491,8 +500,9 @@ def test_adam_types(hip, types, grad_types, lead):
 @pytest.mark.parametrize("wd, decoupled", [(0.0, False), (0.3, False), (0.3, True)])
 @pytest.mark.parametrize("most", [None, 0.3, 1e6])
 @pytest.mark.parametrize("kind", [2.0, math.inf])
-def test_adam_decay_and_clipping(hip, wd, decoupled, most, kind):
-    case = adam_case(30, SIZES, (F32, BF16), (F32, BF16, F32))
+@pytest.mark.parametrize("shapes", [SHORT, SIZES])
+def test_adam_decay_and_clipping(hip, shapes, wd, decoupled, most, kind):
+    case = adam_case(30, shapes, (F32, BF16), (F32, BF16, F32))
     norm = norm64(doubles(case[1]), kind)
     scaled = most if most != 0.3 else 0.3 * norm
     share = 1.0 if most is None else min(1.0, scaled / (norm + 1e-6))
@@ -519,18 +529,21 @@ def test_adam_many_small_tensors_and_a_list_of_counts(hip):
 
 
 @gpu
-def test_adam_with_other_gradients_rate_and_norm_on_the_device(hip):
-    p, g, m, v, step = adam_case(60, [(3, 5)] * 500 + [(70000,)], (F32,), (F32,))
+@pytest.mark.parametrize("shapes", [[(3, 5)] * 500 + [(70000,)], [(3, 5)] * 5 + [(700,)], [(0,)] * 3])
+def test_adam_with_other_gradients_rate_and_norm_on_the_device(hip, shapes):
+    p, g, m, v, step = adam_case(60, shapes, (F32,), (F32,))
     plan = hip.adam(p, None, m, v, step)
     with pytest.raises(ValueError):
         plan.run(1e-2)
-    other = make(66, [(3, 5)] * 500 + [(70000,)], (F32,), 0.3, lead=1)
+    other = make(66, shapes, (F32,), 0.3, lead=1)
     lr = torch.tensor([0.02], device="cuda:0")
     norm = torch.tensor(8.0, device="cuda:0")
     case = (p, other, m, v, step)
     check_adam(hip, *case, plan=plan, lr=lr, grads=other, max_norm=2.0, grad_norm=norm, norm=8.0, share=2.0 / (8.0 + 1e-6))
     check_adam(hip, *case, plan=plan, lr=lr, grads=other)
     for bad in (other[:-1], [t.half() for t in other], [t.cpu() for t in other], p, [t[:1] for t in other]):
+        if bad is not other and not any(t.numel() for t in other) and bad[0].device == other[0].device and len(bad) == len(other) and bad[0].dtype == F32:
+            continue                                                        # nothing to tell empty ones apart by
         with pytest.raises(ValueError):
             plan.run(1e-2, grads=bad)
     with pytest.raises(ValueError):
@@ -540,18 +553,19 @@ def test_adam_with_other_gradients_rate_and_norm_on_the_device(hip):
 @gpu
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
 @pytest.mark.parametrize("most", [None, 1.0])
-def test_adam_skips_or_takes_what_is_not_finite(hip, bad, most):
-    case = adam_case(70, SIZES, (F32, BF16), (F32,))
+@pytest.mark.parametrize("shapes, at", [(SHORT, 5), (SIZES, 9), ([(3,)] * 400, 9), ([(0,)] * 300 + [(7,)], 300)])
+def test_adam_skips_or_takes_what_is_not_finite(hip, shapes, at, bad, most):
+    case = adam_case(70, shapes, (F32, BF16), (F32,))
     p, g, m, v, step = case
-    g[9].reshape(-1)[3] = bad
+    g[at].reshape(-1)[2] = bad
     had = [[t.clone() for t in c] for c in (p, m, v)] + [step.clone()]
     plan = hip.adam(*case)
     norm = plan.run(1e-2, max_norm=most, skip_nonfinite=True, weight_decay=0.1)
     assert not math.isfinite(float(norm))
     assert torch.equal(step, had[3]) and all(torch.equal(a, b) for c, h in zip((p, m, v), had) for a, b in zip(c, h))
     plan.run(1e-2, max_norm=most)
-    assert bool(p[9].isnan().any()) and torch.equal(step, had[3] + 1)
-    g[9].reshape(-1)[3] = 0.5
+    assert bool(p[at].isnan().any()) and torch.equal(step, had[3] + 1)
+    g[at].reshape(-1)[2] = 0.5
     for c, h in zip((p, m, v), had):
         for a, b in zip(c, h):
             a.copy_(b)
