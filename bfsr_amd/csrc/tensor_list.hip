@@ -545,7 +545,7 @@ bool streams(const BfsrListArgs& a, long long bound) { return a.bytes > bound; }
 int launch_parts(const BfsrListArgs& a, int col, bool stream, int sums, float* out, const Hyper* h, Factors* factors, hipStream_t st)
 {
     const auto k = a.max ? stream ? norm_parts_kernel<true, true> : norm_parts_kernel<true, false> : stream ? norm_parts_kernel<false, true> : norm_parts_kernel<false, false>;
-    k<<<sums + (h ? (a.n + TN - 1) / TN : 0), TN, 0, st>>>((const Row*)a.rows, (const int2*)a.chunks, (const void* const*)a.other, col, a.count, sums, (double*)a.work, out, a.n,
+    k<<<sums + (h ? (a.n + TN - 1) / TN : 0), TN, 0, st>>>((const Row*)a.rows, (const int2*)a.chunks, h ? (const void* const*)a.other : nullptr, col, a.count, sums, (double*)a.work, out, a.n,
                                                         h ? *h : Hyper{}, factors);
     return (int)hipGetLastError();
 }
@@ -565,7 +565,7 @@ extern "C" int bfsr_list_write(const void* const* const* cols, int ncols, const 
     long long count = 0;
     for (int k = 0; k < n; ++k) {
         const int t = types[k] & 15, g = types[k] >> 4;
-        if (sizes[k] < 0 || t > BFSR_LIST_BF16 || g < 0 || g > BFSR_LIST_BF16) return -1;
+        if (sizes[k] < 0 || sizes[k] > ((long long)CHUNK << 24) || t > BFSR_LIST_BF16 || g < 0 || g > BFSR_LIST_BF16) return -1;
         for (int c = 0; c < ncols; ++c)
             if (!cols[c] || (sizes[k] && !cols[c][k])) return -1;
         if (ncols == 5 && !cols[4][k]) return -1;

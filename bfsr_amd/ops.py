@@ -128,13 +128,13 @@ def list_column(tensors, device, what, types=LIST_TYPES, like=None, alias=True):
 
 def _versions(tensors):
     """Of `tensors`, one for each version counter: views of one tensor share it, and there may be hundreds of them."""
-    bases, got = set(), []
+    bases, got = {}, []
     for t in tensors:
         base = t._base
         if base is not None:
             if id(base) in bases:
                 continue
-            bases.add(id(base))
+            bases[id(base)] = base                     # held, so that its id stays its own
         if not t.is_inference():
             got.append(t.detach())
     return got

@@ -63,13 +63,13 @@ class Adam(torch.optim.Optimizer):
             self.__dict__.setdefault(name, value)
         for group in self.param_groups:
             group.setdefault("decoupled_weight_decay", False)
-            if group.get("amsgrad") or group.get("maximize"):
-                raise ValueError("Adam: amsgrad and maximize are not supported")
 
     def __getstate__(self):
         return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm, skip_nonfinite=self.skip_nonfinite)
 
     def load_state_dict(self, state_dict):
+        if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
+            raise ValueError("Adam: amsgrad and maximize are not supported")
         super().load_state_dict(state_dict)
         # torch casts loaded moments to the parameter's type and leaves `step` where it was: take both from the dict as they are
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]

@@ -99,7 +99,7 @@ def test_c_entries_refuse_before_a_launch():
     assert write(sizes=(C.c_longlong * 1)(-1)) == write(types=(C.c_int * 1)(3)) == write(types=(C.c_int * 1)(3 << 4)) == write(types=(C.c_int * 1)(-1)) == -1
     assert write(c=(C.c_void_p * 1)(0)) == write(c=(C.c_void_p * 1)(C.addressof(null))) == -1
     assert write(ncols=5, sizes=(C.c_longlong * 1)(0), c=(C.c_void_p * 5)(*[C.addressof(one)] * 4 + [C.addressof(null)])) == -1
-    assert write(sizes=(C.c_longlong * 1)(chunk << 24)) == -1
+    assert write(sizes=(C.c_longlong * 1)(chunk << 24)) == write(sizes=(C.c_longlong * 1)((1 << 63) - 1)) == -1
     assert lib.bfsr_pointer_write(None, 1, 4096, None) == lib.bfsr_pointer_write(one, 0, 4096, None) == lib.bfsr_pointer_write(one, 1, None, None) == -1
     a, h = _lib.BfsrListArgs(), _lib.BfsrAdamArgs()
     good = dict(rows=4096, chunks=4096, n=1, count=1, chunk=chunk, work=4096, norm=4096)
@@ -143,7 +143,8 @@ def test_optimizer_host_side():
     twin = copy.deepcopy(own)
     assert twin.max_grad_norm == 2.0 and twin._plans == {} and twin._ops is None
     with pytest.raises(ValueError):
-        own.load_state_dict(torch.optim.Adam(q, amsgrad=True).state_dict())
+        own.load_state_dict(torch.optim.Adam(q, lr=7.0, amsgrad=True).state_dict())
+    assert own.param_groups[0]["lr"] == 0.1 and float(own.state[p[0]]["step"]) == 2.0
     p[0].grad = torch.ones_like(p[0])
     with pytest.raises(ValueError):
         optim.Adam(p).step()                                                # no CPU path
@@ -701,6 +702,9 @@ def test_optimizer_against_torch_in_64_bits(hip, decoupled, groups):
         net(torch.randn(2, 3, 16, 16, generator=torch.Generator().manual_seed(k)).cuda()).square().mean().backward()
         if k == 2:
             net.c.bias.grad = None
+        if k == 1:                                                          # gradients in another order than their parameters
+            net.b.weight.grad = net.b.weight.grad.contiguous()
+            net.a.weight.grad = net.a.weight.grad.to(memory_format=torch.channels_last)
         for a, b in zip(net.parameters(), ref.parameters()):
             b.grad = None if a.grad is None else a.grad.cpu().double()
         kept = [None if p.grad is None else p.grad.clone() for p in net.parameters()]
