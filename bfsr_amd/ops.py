@@ -169,6 +169,9 @@ class Spans(object):
         return bool(((k < self.start.size) & (size > 0) & (self.start[near] < at + size)).any())
 
 
+_captured = {}             # tables that captured graphs read, for good: nothing tells when a graph is gone
+
+
 class ListTable(object):
     """The device table of a list of tensors (HipOps.tensor_list, HipOps.adam).  It names the memory that the tensors had when it was made.
 
@@ -214,7 +217,7 @@ class ListTable(object):
             if stream != self.stream:
                 self.table.record_stream(torch.cuda.current_stream(i))
             if torch.cuda.is_current_stream_capturing():
-                ops._captured_tables[id(self.table)] = self.table      # a graph reads it at every replay, whatever becomes of the list
+                _captured[self.rows] = self.table      # a graph reads it at every replay, whatever becomes of the list
         other, work = None, self.work
         if grads is not None:
             other = torch.empty(self.n, dtype=torch.int64, device=self.device)
@@ -406,7 +409,6 @@ class HipOps(object):
         self.range_flag = torch.zeros(1, dtype=torch.int32, device=self.device)
         # guard.run_guarded: passes re-run under the bf16x3 split because the fp16 pair met a value outside its range (0 in normal operation)
         self.fallbacks, self._fallback, self._guard_depth, self._range_scratch = 0, None, 0, None
-        self._captured_tables = {}                       # tables of tensor lists that captured graphs read
 
     def cu_count(self):
         """Compute units of the device (the persistent kernels launch one workgroup per CU)."""
