@@ -516,6 +516,31 @@ def test_adam_numbers(hip, betas, eps, lr):
     check_adam(hip, *adam_case(40, SIZES, (F32,), (F32,)), betas=betas, eps=eps, lr=lr)
 
 
+LARGE = [(3500017,), (33,), (2999, 1001), (0,), (3000000,), (1,)]           # more than the shared cache is counted on for: read and written past it
+
+
+@gpu
+@pytest.mark.parametrize("lead", [0, 1])
+@pytest.mark.parametrize("kind", [2.0, math.inf])
+def test_large_lists(hip, kind, lead):
+    ts = make(45, LARGE * 3, (F32, BF16, F16, F32), 0.1, lead)
+    want = doubles(ts)
+    norm = norm64(want, kind)
+    into = [torch.full_like(t, 7.0) for t in ts]
+    tl = hip.tensor_list(ts, out=into)
+    assert tl.bytes > 128 << 20
+    near_norm(hip.grad_norm(tl, kind), norm, 1 << 25)
+    near_norm(hip.clip_grads(tl, norm / 3, kind), norm, 1 << 25)
+    near_clipped(into, want, norm / 3 / (norm + 1e-6))
+    del ts, into, tl, want
+    case = adam_case(46, LARGE, (F32, F32, BF16, F32), (F32, BF16, F16, F32), lead)
+    norm = norm64(doubles(case[1]), kind)
+    plan = check_adam(hip, *case, share=0.5 * norm / (norm + 1e-6), norm=norm, max_norm=0.5 * norm, norm_type=kind, wd=0.1, decoupled=bool(lead))
+    assert plan.bytes > 128 << 20
+    base = case[0][0]._base
+    assert float(base.reshape(-1)[-1]) == 77.0 and (not lead or float(base.reshape(-1)[0]) == 77.0)
+
+
 @gpu
 def test_adam_many_small_tensors_and_a_list_of_counts(hip):
     p, g, m, v, step = adam_case(50, [(3, 5)] * 700 + [(70000,)], (F32,), (F32,))
