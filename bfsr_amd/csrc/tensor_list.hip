@@ -240,6 +240,7 @@ __device__ __forceinline__ void begin_row(const Row& r, const Hyper& h, Factors*
     *f = {(float)(lr / (1.0 - power(h.beta1, (unsigned)t))), (float)(1.0 / sqrt(1.0 - power(h.beta2, (unsigned)t))), (float)(1.0 - lr * h.weight_decay), had};
 }
 
+// A thread a row: 2.5 us for 8 rows, 4.8 for 702, which is three loads that depend on each other.
 __global__ __launch_bounds__(T) void adam_begin_kernel(const Row* __restrict__ rows, int n, Hyper h, Factors* __restrict__ factors)
 {
     const int k = blockIdx.x * T + threadIdx.x;
@@ -272,6 +273,7 @@ __device__ __forceinline__ double sum_chunks(const Row* __restrict__ rows, const
     return wave_join<MAX>((threadIdx.x & 63) < WAVES ? part[threadIdx.x & 63] : 0.0);
 }
 
+// Memory bounds it: 614 MB of fp32 in 93 us (6.6 TB/s, streaming), 77 MB of fp16 in 14 us (5.4), 18 MB in 6.0 us, where its start and end are most of it.
 // One part of the norm for each of the first `sums` workgroups (with one, the norm itself); those behind them, if any, begin a step of Adam.
 template <bool MAX, bool STREAM>
 __global__ __launch_bounds__(TN) void norm_parts_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other,
@@ -290,6 +292,7 @@ __global__ __launch_bounds__(TN) void norm_parts_kernel(const Row* __restrict__ 
     }
 }
 
+// 1.5 us; 3.8 where what came before has emptied the caches.
 __global__ __launch_bounds__(64) void norm_finish_kernel(Norm f)
 {
     const double norm = whole(f);
@@ -341,7 +344,7 @@ __device__ __forceinline__ void clip_one(const Row* __restrict__ rows, const int
 }
 
 // One chunk for each wave, and then the wave ends: one that went on to another chunk would wait for its stores before the next loads count as arrived.
-// Chunks are taken from the end, where the cache holds what the norm has read last.
+// Chunks are taken from the end, where the cache holds what the norm has read last.  Memory bounds it: 307 MB of bf16 read and written in 98 us (6.2 TB/s), 18 MB of fp32 in 7.6.
 template <bool STREAM>
 __global__ __launch_bounds__(T) void clip_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, int count, Norm f)
 {
@@ -439,7 +442,9 @@ __device__ __forceinline__ void adam_one(const Row* __restrict__ rows, const int
 // The share of a step, or -1 where it is skipped: its norm is infinite or NaN, and the caller asked for that.
 __device__ __forceinline__ float share_of_step(const Norm& f, const Hyper& h, double norm) { return h.skip && !(norm <= 1.7976931348623157e308) ? -1.f : share_of(f, norm); }
 
-// One chunk for each workgroup; the last workgroup sees to the norm's output, and to the counts of a step that is skipped.
+// One chunk for each workgroup: two loads of 16 bytes from each of four arrays under way a thread, about fifty instructions an element, a division and a root among them.  Memory bounds
+// it: 153 M fp32 parameters (28 bytes each, none moved twice) in 705 us (6.1 TB/s), 16.7 M bf16 ones (22 bytes) in 62 us (5.9); 512 threads a chunk 2 % less to 2 % more.
+// The workgroup behind the chunks sees to the norm's output, and to the counts of a step that is skipped.
 template <bool STREAM>
 __global__ __launch_bounds__(T) void adam_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other, int count, int n,
                                                  Norm f, Hyper h, const Factors* __restrict__ factors)
@@ -483,7 +488,7 @@ __global__ __launch_bounds__(TN) void adam_alone_kernel(const Row* __restrict__ 
 }
 
 // ---- the table: rows and chunks travel to the device as kernel arguments.  No host buffer has to outlive the call, nothing waits for the stream, and a
-// captured graph holds what it needs.
+// captured graph holds what it needs.  A launch takes 149 rows (one column), 112 (two) or 64 (five) and 2.4 us.
 template <int COLS>
 struct Entry { const void* p[COLS]; long long n; int types, first; };          // first: the row's first chunk
 constexpr int ARGS = 3584;                                                     // bytes of a kernel's arguments that hold entries, of 4096
