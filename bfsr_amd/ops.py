@@ -140,8 +140,18 @@ def _versions(tensors):
     return got
 
 
-def _addresses(tensors):
-    return np.array([t.data_ptr() for t in tensors], dtype=np.int64)
+def _held(t, what):
+    """Refuses a tensor whose storage no longer holds its elements (freed or shrunk by resize_): what it calls its address is then an offset, or 0."""
+    if t.numel() and t.untyped_storage().nbytes() < (t.storage_offset() + t.numel()) * t.itemsize:
+        raise ValueError("%s: its storage has been freed (%d bytes left)" % (what, t.untyped_storage().nbytes()))
+
+
+def _addresses(tensors, what="tensors"):
+    """Where dense tensors begin.  Offsets into freed storage are far below 2^40 (the card holds 2^38 bytes), so only what is there is looked at: 0.15 us a tensor otherwise."""
+    at = np.array([t.data_ptr() for t in tensors], dtype=np.int64)
+    for k in np.flatnonzero(at < 1 << 40):
+        _held(tensors[k], "%s[%d]" % (what, k))
+    return at
 
 
 def _bytes(tensors):
@@ -270,7 +280,7 @@ class TensorList(ListTable):
         replay.  Such a list is never handed out: kept, it could be read where its table has not been written."""
         dev = ops._index_device()
         tensors = list_column(tensors, dev, "tensor_list", alias=False)
-        at, nbytes = _addresses(tensors), _bytes(tensors)
+        at, nbytes = _addresses(tensors, "tensor_list"), _bytes(tensors)
         # aliases hold the memory that the table names, whatever becomes of the tensors
         self.tensors, self.out, cols = [t.detach() for t in tensors], None, [at]
         if out is None:
@@ -280,7 +290,7 @@ class TensorList(ListTable):
             self.out = [t.detach() for t in out]
             if any(a.dtype != b.dtype for a, b in zip(tensors, out)):
                 raise ValueError("tensor_list.out: need the types of the tensors")
-            cols.append(_addresses(out))
+            cols.append(_addresses(out, "tensor_list.out"))
             if Spans(cols[1], nbytes, "tensor_list.out").meet(at, nbytes):
                 raise ValueError("tensor_list.out: overlaps the tensors (leave `out` away to write in place)")
         self.written = _versions(tensors if out is None else out)
@@ -311,10 +321,10 @@ class AdamPlan(ListTable):
         self.expect = [(d, t.shape, t.stride()) for d, t in zip(grad_types, params)]      # of a gradient
         sizes = np.array([t.numel() for t in params], dtype=np.int64)
         self.grad_bytes = sizes * np.array([d.itemsize for d in grad_types])
-        at = [_addresses(c) for c in (self.params, self.exp_avg, self.exp_avg_sq, self.step)]
+        at = [_addresses(c, "adam." + name) for c, name in ((self.params, "params"), (self.exp_avg, "exp_avg"), (self.exp_avg_sq, "exp_avg_sq"), (self.step, "step"))]
         size = [_bytes(params), sizes * 4, sizes * 4, np.full_like(sizes, 4)]
         self.spans = Spans(np.concatenate(at), np.concatenate(size), "adam")
-        grad_at = at[0] if grads is None else _addresses(self.grads)
+        grad_at = at[0] if grads is None else _addresses(self.grads, "adam.grads")
         if grads is not None and self.spans.meet(grad_at, self.grad_bytes):
             raise ValueError("adam.grads: overlap what the update writes")
         self.written = _versions(params)
@@ -331,7 +341,7 @@ class AdamPlan(ListTable):
                 return None
             if g.stride() != stride and not (_dense(g) and _order(g) == tuple(s for s, n in zip(stride, shape) if n != 1 and g.numel())):
                 return None
-        return _addresses(grads)
+        return _addresses(grads, "adam.grads")
 
     def run(self, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled=False, max_norm=None, norm_type=2.0, grad_norm=None, skip_nonfinite=False, grads=None):
         """One step: the counts go up by one, moments and parameters are updated in place.  Nothing waits for the device; may be captured.

@@ -1,0 +1,122 @@
+"""The end of a training step in the calls around its kernels (ops.ListTable, bfsr_amd.optim): freed memory, captured graphs, checkpoints, groups, changing sets of gradients.
+
+`host` runs the host side of the operators on CPU tensors: the table, the checks and the calls as they are, without the kernels."""
+import contextlib
+import math
+import types
+
+import pytest
+import torch
+
+from bfsr_amd import ops as O, optim
+
+CPU = torch.device("cpu")
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _grad():
+    """Other test modules turn gradients off for the whole process."""
+    with torch.enable_grad():
+        yield
+
+
+class Lib(object):
+    """The C entries that a table needs, and a record of the calls."""
+
+    def __init__(self):
+        self.calls, self.gone, self.tickets = [], set(), 0
+
+    def bfsr_list_chunk(self, total):
+        return 2048
+
+    def bfsr_list_work(self, n):
+        return 2048 + 16 * n
+
+    def bfsr_norm_work(self, count):
+        return 0
+
+    def __getattr__(self, name):
+        def entry(*args):
+            self.calls.append((name, args))
+            return 0
+        return entry
+
+
+class Host(object):
+    """An ops object whose launches are only recorded."""
+
+    def __init__(self):
+        self.lib, self.device, self._keylog, self.profile_keys = Lib(), CPU, None, None
+        self.tensor_list, self.adam = (lambda *a, **k: self.made(O.TensorList(self, *a, **k))), (lambda *a: self.made(O.AdamPlan(self, *a)))
+        self.plans = 0
+
+    def made(self, table):
+        self.plans += 1
+        return table
+
+    def _index_device(self):
+        return CPU
+
+    clip_grads, grad_norm, _listed, _norm_out = O.HipOps.clip_grads, O.HipOps.grad_norm, O.HipOps._listed, O.HipOps._norm_out
+
+
+@pytest.fixture
+def host(monkeypatch):
+    stream = types.SimpleNamespace(cuda_stream=0, synchronize=lambda: None)
+    ops = Host()
+    ops.capturing = False
+    for name, value in (("device", lambda d: contextlib.nullcontext()), ("is_current_stream_capturing", lambda: ops.capturing), ("current_stream", lambda d=None: stream),
+                        ("current_device", lambda: None), ("synchronize", lambda d=None: None)):
+        monkeypatch.setattr(torch.cuda, name, value)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 0, raising=False)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: t.device.index, raising=False)       # None on the CPU, like the device's index
+    monkeypatch.setattr(optim, "_ops_of", lambda t, ops_=None: ops_ or ops)
+    yield ops
+
+
+def make(shapes=((4,), (3, 5)), dtype=torch.float32):
+    new = lambda: [torch.randn(s) for s in shapes]                  # noqa: E731
+    return [t.to(dtype) for t in new()], [t.to(dtype) for t in new()], [t * 0 for t in new()], [t * 0 for t in new()], torch.zeros(len(shapes))
+
+
+# ---- memory that is no longer there
+def freed(shape=(4,), offset=0):
+    """A tensor whose storage has been given back, as sharded training does between uses."""
+    base = torch.ones(64)
+    t = base[offset:offset + math.prod(shape)].view(shape)
+    base.untyped_storage().resize_(0)
+    return t
+
+
+@pytest.mark.parametrize("offset", [0, 8])
+def test_freed_storage_is_refused(host, offset):
+    """Its address is an offset, which no kernel may follow."""
+    t = freed(offset=offset)
+    assert t.data_ptr() == 4 * offset
+    with pytest.raises(ValueError, match="freed"):
+        O._addresses([torch.ones(4), t])
+    with pytest.raises(ValueError, match="freed"):
+        host.tensor_list([t])
+    with pytest.raises(ValueError, match="freed"):
+        host.tensor_list([torch.ones(4)], out=[t])
+    p, g, m, v, step = make(((4,),))
+    for args in (([t], g, m, v, step), (p, [t], m, v, step), (p, g, [t], v, step), (p, g, m, [t], step), (p, g, m, v, [freed((), offset)])):
+        with pytest.raises(ValueError, match="freed"):
+            host.adam(*args)
+    plan = host.adam(p, None, m, v, step)
+    plan.run(0.1, grads=g)
+    with pytest.raises(ValueError, match="freed"):
+        plan.run(0.1, grads=[t])
+    assert len([c for c in host.lib.calls if c[0] == "bfsr_adam_step"]) == 1
+    w = torch.nn.Parameter(torch.ones(4))
+    opt = optim.Adam([w], ops=host)
+    w.grad = t
+    with pytest.raises(ValueError, match="freed"):
+        opt.step()
+    O._addresses([torch.zeros(0), torch.zeros(3, 0)])               # nothing to be held
+    shrunk = torch.ones(64)
+    shrunk.untyped_storage().resize_(128)
+    with pytest.raises(ValueError, match="freed"):
+        O._held(shrunk, "x")
+    O._held(shrunk[:32], "x")
