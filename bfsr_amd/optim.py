@@ -104,12 +104,14 @@ class Adam(torch.optim.Optimizer):
             held = None
         found = None if held is None else held[2].fit(grads)
         if found is None:
-            grads = [g if _order(g) == _order(p) else torch.empty_like(p, dtype=g.dtype).copy_(g) for p, g in zip(params, grads)]
+            grads = [g if _order(g) == _order(p) and not g.is_neg() else torch.empty_like(p, dtype=g.dtype).copy_(g) for p, g in zip(params, grads)]
             found = None if held is None else held[2].fit(grads)
         if found is None:
             bring = all(g.dtype == p.dtype for p, g in zip(params, grads))       # the plan holds no gradients, which zero_grad may want to free
             plan = ops.adam(params, None if bring else grads, *[[s[k] for s in state] for k in ("exp_avg", "exp_avg_sq", "step")])
             held, found = (ops, where, plan), plan.fit(grads)
+            if found is None:                        # without addresses the plan would go by its own column, which may be the parameters
+                raise ValueError("Adam: gradients that do not go with their parameters")
             self._plans[at] = held
         return held[2], grads, found
 

@@ -120,3 +120,44 @@ def test_freed_storage_is_refused(host, offset):
     with pytest.raises(ValueError, match="freed"):
         O._held(shrunk, "x")
     O._held(shrunk[:32], "x")
+
+
+# ---- gradients
+def conjugated(values, device="cpu"):
+    """A gradient of one element behind a lazy minus sign."""
+    g = torch.complex(torch.zeros(1), -torch.tensor([values])).to(device).conj().imag
+    assert g.is_neg() and float(g) == values
+    return g
+
+
+def test_lazily_negated_gradients_are_read(host):
+    """A step without the gradients' addresses would take the parameters for them."""
+    w = torch.nn.Parameter(torch.ones(1))
+    opt = optim.Adam([w], ops=host)
+    for _ in range(2):
+        host.lib.calls.clear()
+        w.grad = conjugated(0.25)
+        opt.step()
+        assert [c[0] for c in host.lib.calls if "write" in c[0] or "step" in c[0]][-2:] == ["bfsr_pointer_write", "bfsr_adam_step"]
+
+
+def test_gradients_that_do_not_go_with_their_parameters_are_refused(host, monkeypatch):
+    w = torch.nn.Parameter(torch.ones(1))
+    w.grad = torch.ones(1)
+    opt = optim.Adam([w], ops=host)
+    monkeypatch.setattr(O.AdamPlan, "fit", lambda self, grads: None)
+    with pytest.raises(ValueError):
+        opt.step()
+
+
+@gpu
+def test_lazily_negated_gradients_on_the_gpu():
+    got = []
+    for lazy in (False, True):
+        w = torch.nn.Parameter(torch.full((1,), 2.0, device="cuda:0"))
+        opt = optim.Adam([w], lr=0.1)
+        for g in (0.25, -0.5):
+            w.grad = conjugated(g, "cuda:0") if lazy else torch.tensor([g], device="cuda:0")
+            opt.step()
+        got.append((float(w.detach()), float(opt.state[w]["exp_avg"])))
+    assert got[0] == got[1] and got[0][1] == pytest.approx(0.9 * 0.025 - 0.05, abs=1e-8)
