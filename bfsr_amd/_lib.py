@@ -293,6 +293,8 @@ SYMBOLS = {
     "bfsr_grad_norm": (_I, [C.POINTER(BfsrListArgs), _VP]),
     "bfsr_clip_grads": (_I, [C.POINTER(BfsrListArgs), _F, _VP]),
     "bfsr_adam_step": (_I, [C.POINTER(BfsrListArgs), C.POINTER(BfsrAdamArgs), _VP]),
+    "bfsr_capture_ticket": (_I, [_VP, C.POINTER(_VP)]),
+    "bfsr_capture_gone": (_I, [_VP]),
     "bfsr_conv2d_direct": (_I, [_VP, _LL, _VP, _VP, _VP, _LL, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _VP]),
 }
 

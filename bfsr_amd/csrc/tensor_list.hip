@@ -10,6 +10,8 @@
 // the element's own alignment: the vector types below say so and gfx950's global loads of 8 and 16 bytes take it.
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
+#include <atomic>
+#include <new>
 #include "../../include/bfsr_hip.h"
 #include "launch_util.h"
 
@@ -653,4 +655,34 @@ extern "C" int bfsr_adam_step(const BfsrListArgs* a, const BfsrAdamArgs* h, void
     (past ? adam_kernel<true> : adam_kernel<false>)<<<a->count + 1, T, 0, st>>>((const Row*)a->rows, (const int2*)a->chunks, (const void* const*)a->other, a->count, a->n,
                                                    Norm{(const double*)a->work, own ? sums_of(a->count) : 0, a->max, given, norm ? a->norm : nullptr, max_norm}, hy, factors);
     return (int)hipGetLastError();
+}
+
+// ---- the life of a captured graph.  The graph owns a reference to a ticket, and so does every executable made from it; the runtime says when the last one is gone, on a thread of
+// its choice and perhaps at the process's end, so that notice sets a flag in plain memory and nothing else.
+extern "C" int bfsr_capture_ticket(void* stream, void** ticket)
+{
+    if (!ticket) return -1;
+    *ticket = nullptr;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    hipGraph_t graph = nullptr;
+    hipError_t err = hipStreamGetCaptureInfo_v2((hipStream_t)stream, &status, nullptr, &graph, nullptr, nullptr);
+    if (err != hipSuccess || status != hipStreamCaptureStatusActive || !graph) return (int)err;
+    std::atomic<int>* gone = new (std::nothrow) std::atomic<int>(0);
+    if (!gone) return (int)hipErrorOutOfMemory;
+    hipUserObject_t object = nullptr;
+    err = hipUserObjectCreate(&object, gone, [](void* flag) { ((std::atomic<int>*)flag)->store(1, std::memory_order_release); }, 1, hipUserObjectNoDestructorSync);
+    if (err != hipSuccess) { delete gone; return (int)err; }
+    err = hipGraphRetainUserObject(graph, object, 1, hipGraphUserObjectMove);
+    if (err != hipSuccess) return (int)err;                        // the flag stays the object's
+    *ticket = gone;
+    return 0;
+}
+
+extern "C" int bfsr_capture_gone(void* ticket)
+{
+    std::atomic<int>* gone = (std::atomic<int>*)ticket;
+    if (!gone) return -1;
+    if (!gone->load(std::memory_order_acquire)) return 0;
+    delete gone;
+    return 1;
 }

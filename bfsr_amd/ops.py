@@ -8,6 +8,7 @@ test double with the same interface to exercise the host-side schedule without a
 import ctypes as C
 import math
 import os
+import threading
 
 import numpy as np
 import torch
@@ -179,7 +180,25 @@ class Spans(object):
         return bool(((k < self.start.size) & (size > 0) & (self.start[near] < at + size)).any())
 
 
-_captured = {}             # tables that captured graphs read, for good: nothing tells when a graph is gone
+_captured = []             # of captured calls: the graph's ticket, the table, and what else its replays read
+_captured_lock = threading.Lock()
+
+
+def _hold(lib, stream, table, *reads):
+    """Keeps a table, with the memory that it names, and `reads` for as long as the graph exists into which `stream` is being captured."""
+    ticket = C.c_void_p()
+    _lib.check(lib.bfsr_capture_ticket(stream, C.byref(ticket)), "capture_ticket")
+    with _captured_lock:
+        _captured.append((ticket.value, table, reads))
+
+
+def _let_go(lib):
+    """Lets go of what the graphs that are gone by now have needed."""
+    with _captured_lock:
+        gone = [k for k, held in enumerate(_captured) if held[0] is not None and lib.bfsr_capture_gone(held[0])]
+        over = [_captured.pop(k) for k in reversed(gone)]
+    for device in {held[1].device for held in over}:
+        torch.cuda.synchronize(device)                     # a graph may go while its last replay still runs
 
 
 class ListTable(object):
@@ -204,6 +223,8 @@ class ListTable(object):
         with torch.cuda.device(self.device):
             if not once and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("tensor list: make it before the capture begins (its table is written once, not at every replay)")
+            if not once:
+                _let_go(ops.lib)
             stream = torch.cuda.current_stream(self.device)
             self.stream = stream.cuda_stream
             # behind the table: scratch for what writes the tensors, since two such calls cannot run at the same time anyway.  A norm gets its own for each call
@@ -218,18 +239,18 @@ class ListTable(object):
             if not once:
                 stream.synchronize()               # from here on the table may be read on any stream
 
-    def call(self, name, fn, kind, norm, *more, grads=None):
-        """One C call over the list on the current stream; `grads`: addresses in place of the table's gradients."""
+    def call(self, name, fn, kind, norm, *more, grads=None, reads=()):
+        """One C call over the list on the current stream; `grads`: addresses in place of the table's gradients; `reads`: tensors that `more` names by their addresses."""
         i = self.device.index
         if torch.cuda.current_device() != i:       # a launch needs its device to be the current one
             with torch.cuda.device(i):
-                return self.call(name, fn, kind, norm, *more, grads=grads)
+                return self.call(name, fn, kind, norm, *more, grads=grads, reads=reads)
         ops, stream = self.ops, torch._C._cuda_getCurrentRawStream(i)
         if not self.once:
             if stream != self.stream:
                 self.table.record_stream(torch.cuda.current_stream(i))
             if torch.cuda.is_current_stream_capturing():
-                _captured[self.rows] = self.table      # a graph reads it at every replay, whatever becomes of the list
+                _hold(ops.lib, stream, self, *reads)   # the table, and the memory that it names, whatever becomes of the list and its tensors
         other, work = None, self.work
         if grads is not None:
             other = torch.empty(self.n, dtype=torch.int64, device=self.device)
@@ -353,6 +374,7 @@ class AdamPlan(ListTable):
         skip_nonfinite    where the norm is infinite or NaN, nothing changes, step counts included
         grads             the gradients of this step, where the plan has none or they stand elsewhere than its own (shapes and orders of the axes of the
                           parameters, types of the plan's gradients)
+        A graph into which a step is captured holds all that the plan names, `lr` and `grad_norm`; gradients given here are the caller's to keep.
 
         Returns the norm before clipping (0-d, on the device) with max_norm or skip_nonfinite, None otherwise."""
         at = None
@@ -366,7 +388,7 @@ class AdamPlan(ListTable):
 
     def _run(self, grads, lr, betas, eps, weight_decay, decoupled, max_norm, norm_type, grad_norm, skip_nonfinite):
         """run() with the addresses that fit() gave, or None."""
-        dev, at = self.device, None
+        dev, at, reads = self.device, None, [t.detach() for t in (lr, grad_norm) if isinstance(t, torch.Tensor)]
         if isinstance(lr, torch.Tensor):
             at, lr = _one_float(lr, dev, "adam.lr").data_ptr(), 0.0
         beta1, beta2 = betas
@@ -383,7 +405,7 @@ class AdamPlan(ListTable):
                               -1.0 if max_norm is None else _at_least_0(max_norm, "adam.max_norm"), given, bool(skip_nonfinite))
         if grads is not None and self.spans.meet(grads, self.grad_bytes):
             raise ValueError("adam.grads: overlap what the update writes")
-        self.call("adam_step", self.ops.lib.bfsr_adam_step, kind, norm, h, grads=grads)
+        self.call("adam_step", self.ops.lib.bfsr_adam_step, kind, norm, h, grads=grads, reads=reads)
         torch.autograd.graph.increment_version(self.written)
         return norm
 
@@ -467,7 +489,8 @@ class HipOps(object):
 
         The handle stands for the memory that the tensors have now, and holds it: their values are read at each call, but a gradient that is made anew (zero_grad
         with set_to_none) needs a new handle, and so does one whose storage is resized.  Making one waits for the current stream; it may then be used on any
-        stream, and in graphs, which have to be captured after it was made.  Two calls that write the same tensors cannot run at the same time; norms can."""
+        stream, and in graphs, which have to be captured after it was made and hold the handle, and so that memory, as long as they exist.  Two calls that write the
+        same tensors cannot run at the same time; norms can."""
         return TensorList(self, tensors, out)
 
     def grad_norm(self, tensors, norm_type=2.0, out=None):
@@ -483,7 +506,7 @@ class HipOps(object):
     def clip_grads(self, tensors, max_norm, norm_type=2.0):
         """Multiplies a tensor_list, in place or into its `out`, or a plain list of tensors in place, by min(1, max_norm / (norm + 1e-6)); returns the norm
         before (0-d float32, on the device).  An infinite norm makes finite gradients 0, a NaN makes all NaN, as the quotient does.  Products are rounded
-        once, to the tensor's type."""
+        once, to the tensor's type.  What a graph is captured with stays allocated where it is a handle's; a plain list's tensors are the caller's to keep."""
         kind, max_norm, tensors = _norm_type(norm_type), _at_least_0(max_norm, "clip_grads.max_norm"), self._listed(tensors)
         norm = self._norm_out(tensors, None)
         if tensors.n:

@@ -634,6 +634,10 @@ int bfsr_pointer_write(const void* const* from, int n, void* to, void* stream);
 int bfsr_grad_norm(const BfsrListArgs* a, void* stream);
 int bfsr_clip_grads(const BfsrListArgs* a, float max_norm, void* stream);
 int bfsr_adam_step(const BfsrListArgs* a, const BfsrAdamArgs* h, void* stream);
+/* A graph reads tables and tensors at every replay.  bfsr_capture_ticket: where `stream` is being captured, a ticket of that graph (else NULL); bfsr_capture_gone: 0 while the
+ * graph, or an executable made from it, exists; 1 when all are gone, and the ticket with them (a work item that the device still has may not be over). */
+int bfsr_capture_ticket(void* stream, void** ticket);
+int bfsr_capture_gone(void* ticket);
 
 #ifdef __cplusplus
 }

@@ -2,13 +2,15 @@
 
 `host` runs the host side of the operators on CPU tensors: the table, the checks and the calls as they are, without the kernels."""
 import contextlib
+import gc
 import math
 import types
 
 import pytest
 import torch
+from torch.multiprocessing.reductions import StorageWeakRef
 
-from bfsr_amd import ops as O, optim
+from bfsr_amd import _lib, ops as O, optim
 
 CPU = torch.device("cpu")
 gpu = pytest.mark.gpu
@@ -35,6 +37,14 @@ class Lib(object):
 
     def bfsr_norm_work(self, count):
         return 0
+
+    def bfsr_capture_ticket(self, stream, ticket):
+        self.tickets += 1
+        ticket._obj.value = self.tickets
+        return 0
+
+    def bfsr_capture_gone(self, ticket):
+        return int(ticket in self.gone)
 
     def __getattr__(self, name):
         def entry(*args):
@@ -72,6 +82,7 @@ def host(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 0, raising=False)
     monkeypatch.setattr(torch.Tensor, "get_device", lambda t: t.device.index, raising=False)       # None on the CPU, like the device's index
     monkeypatch.setattr(optim, "_ops_of", lambda t, ops_=None: ops_ or ops)
+    monkeypatch.setattr(O, "_captured", type(O._captured)())
     yield ops
 
 
@@ -161,3 +172,70 @@ def test_lazily_negated_gradients_on_the_gpu():
             opt.step()
         got.append((float(w.detach()), float(opt.state[w]["exp_avg"])))
     assert got[0] == got[1] and got[0][1] == pytest.approx(0.9 * 0.025 - 0.05, abs=1e-8)
+
+
+# ---- graphs: what a replay reads and writes lives as long as the graph
+def refs(tensors):
+    return [StorageWeakRef(t.untyped_storage()) for t in tensors]
+
+
+def test_captured_calls_hold_their_memory(host):
+    p, g, m, v, step = make()
+    out = [torch.zeros_like(t) for t in g]
+    lr, norm = torch.tensor(0.1), torch.tensor(2.0)
+    plan, clip = host.adam(p, g, m, v, step), host.tensor_list(g, out=out)
+    held = refs(p + m + v + g + [step, lr, norm])
+    taken = refs(g + out)
+    loose = refs(make()[0])
+    host.capturing = True
+    plan.run(lr, max_norm=1.0, grad_norm=norm)
+    host.clip_grads(clip, 1.0)
+    host.clip_grads([torch.ones(3)], 1.0)                           # a plain list's memory is the caller's to keep
+    host.capturing = False
+    del p, g, m, v, step, out, lr, norm, plan, clip
+    gc.collect()
+    host.tensor_list([torch.ones(3)])
+    assert not any(r.expired() for r in held + taken) and all(r.expired() for r in loose) and len(O._captured) == 2
+    host.lib.gone.add(1)
+    host.tensor_list([torch.ones(3)])                               # the next table finds the first graph gone
+    assert [r.expired() for r in held] == [True] * 6 + [False] * 2 + [True] * 3 and not any(r.expired() for r in taken)
+    host.lib.gone.add(2)
+    host.tensor_list([torch.ones(3)])
+    assert all(r.expired() for r in held + taken) and not O._captured
+
+
+def test_tickets_are_refused():
+    lib = _lib.load()
+    assert lib.bfsr_capture_ticket(None, None) == lib.bfsr_capture_gone(None) == -1
+
+
+@gpu
+def test_a_graph_outlives_its_plan():
+    """Nothing else holds the captured plan's moments, counts and rate: replays still find them, memory that is taken meanwhile stays as it is, and it ends with the graph."""
+    hip = O.HipOps("cuda:0")
+    shapes = [(3000,), (17, 65), (70001,)]
+    new = lambda f: [torch.full(s, f, device="cuda:0") for s in shapes]              # noqa: E731
+    p, g, m, v, step = new(1.0), new(0.5), new(0.0), new(0.0), torch.zeros(3, device="cuda:0")
+    lr = torch.tensor(0.25, device="cuda:0")
+    plan = hip.adam(p, g, m, v, step)
+    before = len(O._captured)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.run(lr, betas=(0.5, 0.5))
+    ends = refs(m + v + [step, lr])
+    del plan, m, v, step, lr
+    gc.collect()
+    junk = [new(7.0) for _ in range(4)] + [[torch.full((k,), 7.0, device="cuda:0") for k in (1, 1, 3, 3)]]
+    hip.tensor_list(g)
+    assert len(O._captured) == before + 1 and not any(r.expired() for r in ends)
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        # a constant gradient: m / (1 - b^t) = g, v / (1 - b^t) = g^2, so each step takes lr away, but for a dozen roundings and eps
+        for t in p:
+            assert float((t - (0.75 - 0.25 * k)).abs().max()) <= 16 * 2.0 ** -24 * (k + 1) + 2e-8 * (k + 1)
+    assert all(float(t.min()) == 7.0 == float(t.max()) for c in junk for t in c)
+    del graph
+    gc.collect()
+    hip.tensor_list(g)
+    assert len(O._captured) == before and all(r.expired() for r in ends)
