@@ -70,6 +70,11 @@ class Adam(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
             raise ValueError("Adam: amsgrad and maximize are not supported")
+        # AdamW did not always write the key: such a group goes on with the decay that it has here
+        groups = [dict(g) for g in state_dict["param_groups"]]
+        for group, here in zip(groups, self.param_groups):
+            group.setdefault("decoupled_weight_decay", here["decoupled_weight_decay"])
+        state_dict = dict(state_dict, param_groups=groups)
         super().load_state_dict(state_dict)
         # torch casts loaded moments to the parameter's type and leaves `step` where it was: take both from the dict as they are
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]

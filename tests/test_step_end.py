@@ -239,3 +239,21 @@ def test_a_graph_outlives_its_plan():
     gc.collect()
     hip.tensor_list(g)
     assert len(O._captured) == before and all(r.expired() for r in ends)
+
+
+# ---- checkpoints
+@pytest.mark.parametrize("written", [True, False])
+@pytest.mark.parametrize("theirs, decoupled", [(torch.optim.AdamW, True), (torch.optim.Adam, False)])
+def test_decay_of_a_loaded_checkpoint(theirs, decoupled, written):
+    """A checkpoint decides between the two decays where it says which one it used; older ones do not, and leave it to the optimizer that loads them."""
+    w = [torch.nn.Parameter(torch.ones(3)) for _ in range(2)]
+    saved = theirs([dict(params=[p], weight_decay=0.1 * (k + 1)) for k, p in enumerate(w)], lr=0.5).state_dict()
+    for k, g in enumerate(saved["param_groups"]):
+        g["decoupled_weight_decay"] = decoupled
+        if not written:
+            del g["decoupled_weight_decay"]
+    opt = optim.Adam([dict(params=[w[0]], decoupled_weight_decay=True), dict(params=[w[1]], decoupled_weight_decay=False)], lr=0.1)
+    opt.load_state_dict(saved)
+    assert [g["decoupled_weight_decay"] for g in opt.param_groups] == ([decoupled] * 2 if written else [True, False])
+    assert [(g["lr"], g["weight_decay"]) for g in opt.param_groups] == [(0.5, 0.1), (0.5, 0.2)]
+    assert all(("decoupled_weight_decay" in g) == written for g in saved["param_groups"])              # the caller's dict stays as it was
