@@ -68,14 +68,25 @@ class Adam(torch.optim.Optimizer):
         return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm, skip_nonfinite=self.skip_nonfinite)
 
     def load_state_dict(self, state_dict):
-        if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
-            raise ValueError("Adam: amsgrad and maximize are not supported")
-        # AdamW did not always write the key: such a group goes on with the decay that it has here
-        groups = [dict(g) for g in state_dict["param_groups"]]
-        for group, here in zip(groups, self.param_groups):
-            group.setdefault("decoupled_weight_decay", here["decoupled_weight_decay"])
-        state_dict = dict(state_dict, param_groups=groups)
-        super().load_state_dict(state_dict)
+        loading = {}
+
+        def last(_, d):
+            """What the program's own hooks have made of the dict."""
+            if any(g.get("amsgrad") or g.get("maximize") for g in d["param_groups"]):
+                raise ValueError("Adam: amsgrad and maximize are not supported")
+            # AdamW did not always write the key: such a group goes on with the decay that it has here
+            groups = [dict(g) for g in d["param_groups"]]
+            for group, here in zip(groups, self.param_groups):
+                group.setdefault("decoupled_weight_decay", here["decoupled_weight_decay"])
+            loading.update(d, param_groups=groups)
+            return loading
+
+        hook = self.register_load_state_dict_pre_hook(last)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            hook.remove()
+        state_dict = loading
         # torch casts loaded moments to the parameter's type and leaves `step` where it was: take both from the dict as they are
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, [p for g in self.param_groups for p in g["params"]]):

@@ -257,3 +257,23 @@ def test_decay_of_a_loaded_checkpoint(theirs, decoupled, written):
     assert [g["decoupled_weight_decay"] for g in opt.param_groups] == ([decoupled] * 2 if written else [True, False])
     assert [(g["lr"], g["weight_decay"]) for g in opt.param_groups] == [(0.5, 0.1), (0.5, 0.2)]
     assert all(("decoupled_weight_decay" in g) == written for g in saved["param_groups"])              # the caller's dict stays as it was
+
+
+def test_hooks_of_loading_see_to_moments_too():
+    w = torch.nn.Parameter(torch.ones(3))
+    saved = optim.Adam([w]).state_dict()
+    saved["state"] = {0: {"step": torch.tensor(4.0), "exp_avg": torch.full((3,), 1.0), "exp_avg_sq": torch.full((3,), 2.0)}}
+    opt = optim.Adam([w], lr=0.1)
+
+    def twice(_, d):
+        d["state"] = {0: {"step": torch.tensor(9.0), "exp_avg": d["state"][0]["exp_avg"] * 2, "exp_avg_sq": d["state"][0]["exp_avg_sq"] * 4}}
+        d["param_groups"] = [dict(g, lr=0.7) for g in d["param_groups"]]
+        return d
+
+    hook = opt.register_load_state_dict_pre_hook(twice)
+    for _ in range(2):
+        opt.load_state_dict(saved)
+        assert [float(opt.state[w][k].max()) for k in ("step", "exp_avg", "exp_avg_sq")] == [9.0, 2.0, 8.0] and opt.param_groups[0]["lr"] == 0.7
+    hook.remove()
+    opt.load_state_dict(saved)
+    assert [float(opt.state[w][k].max()) for k in ("step", "exp_avg", "exp_avg_sq")] == [4.0, 1.0, 2.0] and opt.param_groups[0]["lr"] == 1e-3
