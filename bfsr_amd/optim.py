@@ -44,7 +44,8 @@ class Adam(torch.optim.Optimizer):
     max_grad_norm     clip the gradients of all groups by their global norm, within the update: p.grad is left as it is
     skip_nonfinite    a step whose gradients' norm is infinite or NaN changes nothing, step counts included
     `grad_norm` holds the last step's norm (0-d, on the device) where one of the two is asked for.
-    A group's lr may be a tensor of one float32 on the device; a step captured into a graph then follows it.  Capture after one ordinary step."""
+    A group's lr may be a tensor of one float32 on the device; a step captured into a graph then follows it.  Capture after one ordinary step,
+    and again after load_state_dict: state and rate are new tensors then, and a graph goes on with the old ones, which it holds."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled_weight_decay=False, max_grad_norm=None, skip_nonfinite=False,
                  ops=None):

@@ -277,3 +277,36 @@ def test_hooks_of_loading_see_to_moments_too():
     hook.remove()
     opt.load_state_dict(saved)
     assert [float(opt.state[w][k].max()) for k in ("step", "exp_avg", "exp_avg_sq")] == [4.0, 1.0, 2.0] and opt.param_groups[0]["lr"] == 1e-3
+
+
+@gpu
+def test_a_graph_captured_before_a_checkpoint_is_loaded():
+    """It goes on with the state that it was captured with, beside the new one."""
+    hip = O.HipOps("cuda:0")
+    w = [torch.nn.Parameter(torch.full((n,), 1.0, device="cuda:0")) for n in (5, 70001)]
+    for p in w:
+        p.grad = torch.full_like(p, 0.5)
+    lr = torch.tensor(0.25, device="cuda:0")
+    opt = optim.Adam(w, lr=lr, betas=(0.5, 0.5), ops=hip)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    ends = refs([t for p in w for t in opt.state[p].values()] + [lr])
+    saved = {"state": {k: {"step": torch.tensor(7.0), "exp_avg": torch.zeros_like(p), "exp_avg_sq": torch.ones_like(p)} for k, p in enumerate(w)},
+             "param_groups": [dict(opt.state_dict()["param_groups"][0], lr=torch.tensor(0.0, device="cuda:0"))]}
+    del lr
+    opt.load_state_dict(saved)
+    opt.step()
+    gc.collect()
+    junk = [[torch.full_like(p, 7.0) for p in w] for _ in range(4)] + [[torch.full((2,), 7.0, device="cuda:0") for _ in range(4)]]
+    assert not any(r.expired() for r in ends)
+    state = [{k: t.clone() for k, t in opt.state[p].items()} for p in w]
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, s in zip(w, state):
+            # steps of a constant gradient take the rate away: 0.25 by the ordinary step, none by the loaded rate of 0, 0.25 by each replay
+            assert float((p - (0.5 - 0.25 * k)).abs().max()) <= (16 * 2.0 ** -24 + 2e-8) * (k + 2)
+            assert all(torch.equal(t, opt.state[p][n]) for n, t in s.items()) and float(s["step"]) == 8.0
+    assert all(float(t.min()) == 7.0 == float(t.max()) for c in junk for t in c)
