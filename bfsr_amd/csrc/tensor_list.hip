@@ -134,7 +134,12 @@ template <> struct Acc<false> {
         for (int k = 0; k < Vec<TYPE>::N; ++k) { const double d = (double)Vec<TYPE>::wide(g[k]); a = fma(d, d, a); }
     }
     __device__ __forceinline__ double part() const { return a; }
-    __device__ static double whole(double sum) { return sqrt(sum); }
+    // What 32 bits cannot hold is infinite, as in the norm that the caller gets: whether a list is clipped and skipped as one or by the norm of several is the same then.
+    __device__ static double whole(double sum)
+    {
+        const double norm = sqrt(sum);
+        return isinf((float)norm) ? (double)(float)norm : norm;
+    }
 };
 template <> struct Acc<true> {
     unsigned a = 0;
@@ -442,7 +447,7 @@ __device__ __forceinline__ void adam_one(const Row* __restrict__ rows, const int
 }
 
 // The share of a step, or -1 where it is skipped: its norm is infinite or NaN, and the caller asked for that.
-__device__ __forceinline__ float share_of_step(const Norm& f, const Hyper& h, double norm) { return h.skip && !(norm <= 1.7976931348623157e308) ? -1.f : share_of(f, norm); }
+__device__ __forceinline__ float share_of_step(const Norm& f, const Hyper& h, double norm) { return h.skip && !isfinite(norm) ? -1.f : share_of(f, norm); }
 
 // One chunk for each workgroup: two loads of 16 bytes from each of four arrays under way a thread, about fifty instructions an element, a division and a root among them.  Memory bounds
 // it: 153 M fp32 parameters (28 bytes each, none moved twice) in 705 us (6.1 TB/s), 16.7 M bf16 ones (22 bytes) in 62 us (5.9); 512 threads a chunk 2 % less to 2 % more.

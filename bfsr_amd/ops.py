@@ -371,7 +371,7 @@ class AdamPlan(ListTable):
         weight_decay      added to the gradient as weight_decay * p; `decoupled`: taken off the parameter as lr * weight_decay * p
         max_norm          gradients count as if clip_grads(max_norm, norm_type) had run before; they stay as they are in memory
         grad_norm         the norm to clip by (a tensor of one float32), where it is not this list's own: of several lists, or over ranks
-        skip_nonfinite    where the norm is infinite or NaN, nothing changes, step counts included
+        skip_nonfinite    where the norm, as it is returned, is infinite or NaN, nothing changes, step counts included
         grads             the gradients of this step, where the plan has none or they stand elsewhere than its own (shapes and orders of the axes of the
                           parameters, types of the plan's gradients)
         A graph into which a step is captured holds all that the plan names, `lr` and `grad_norm`; gradients given here are the caller's to keep.
@@ -505,7 +505,7 @@ class HipOps(object):
 
     def clip_grads(self, tensors, max_norm, norm_type=2.0):
         """Multiplies a tensor_list, in place or into its `out`, or a plain list of tensors in place, by min(1, max_norm / (norm + 1e-6)); returns the norm
-        before (0-d float32, on the device).  An infinite norm makes finite gradients 0, a NaN makes all NaN, as the quotient does.  Products are rounded
+        before (0-d float32, on the device).  An infinite norm (one beyond float32 is that, too) makes finite gradients 0, a NaN makes all NaN, as the quotient does.  Products are rounded
         once, to the tensor's type.  What a graph is captured with stays allocated where it is a handle's; a plain list's tensors are the caller's to keep."""
         kind, max_norm, tensors = _norm_type(norm_type), _at_least_0(max_norm, "clip_grads.max_norm"), self._listed(tensors)
         norm = self._norm_out(tensors, None)

@@ -310,3 +310,60 @@ def test_a_graph_captured_before_a_checkpoint_is_loaded():
             assert float((p - (0.5 - 0.25 * k)).abs().max()) <= (16 * 2.0 ** -24 + 2e-8) * (k + 2)
             assert all(torch.equal(t, opt.state[p][n]) for n, t in s.items()) and float(s["step"]) == 8.0
     assert all(float(t.min()) == 7.0 == float(t.max()) for c in junk for t in c)
+
+
+# ---- norms that are not finite
+BIG = 3.0e38                     # two of them: finite gradients of a norm that float32 does not hold
+
+
+@gpu
+@pytest.mark.parametrize("bad", [(BIG, BIG), (math.inf, 0.0), (0.0, -math.inf), (math.nan, 1.0), (1.0, math.nan)])
+@pytest.mark.parametrize("size", [6, 70001])
+@pytest.mark.parametrize("most", [None, 1.0])
+def test_skipped_steps_do_not_depend_on_the_groups(size, bad, most):
+    got = []
+    for groups in (1, 2):
+        torch.manual_seed(3)
+        w = [torch.nn.Parameter(torch.randn(n, device="cuda:0")) for n in (size, 3, size)]
+        opt = optim.Adam([dict(params=w)] if groups == 1 else [dict(params=w[:1]), dict(params=w[1:])], lr=0.01, weight_decay=0.1, max_grad_norm=most, skip_nonfinite=True)
+        for p in w:
+            p.grad = torch.randn_like(p)
+        opt.step()
+        had = [p.detach().clone() for p in w] + [t.clone() for p in w for t in opt.state[p].values()]
+        w[0].grad[size // 2], w[2].grad[1] = bad
+        opt.step()
+        norm = float(opt.grad_norm)
+        assert math.isnan(norm) if any(map(math.isnan, bad)) else norm == math.inf
+        now = [p.detach() for p in w] + [t for p in w for t in opt.state[p].values()]
+        assert all(torch.equal(a, b) for a, b in zip(had, now))
+        w[0].grad[size // 2], w[2].grad[1] = 0.5, 0.25
+        opt.step()
+        assert math.isfinite(float(opt.grad_norm)) and all(float(opt.state[p]["step"]) == 2.0 for p in w)
+        assert all(bool((p.detach() != b).any()) for p, b in zip(w, had))
+        got.append([p.detach() for p in w])
+    # the norm of two groups is rounded to float32 in between: a share off by 2^-24, and an update of at most 10 lr each that is off by a few of those
+    assert all(float((a - b).abs().max()) <= 2 * 10 * 0.01 * 16 * 2.0 ** -24 + 2.0 ** -22 for a, b in zip(*got))
+
+
+@gpu
+@pytest.mark.parametrize("size", [6, 70001])
+def test_norms_beyond_float32_are_infinite_everywhere(size):
+    hip = O.HipOps("cuda:0")
+    new = lambda: [torch.randn(n, generator=torch.Generator().manual_seed(n)).cuda() for n in (size, 3)]               # noqa: E731
+    g = new()
+    g[0][size // 2] = g[1][1] = BIG
+    assert float(hip.grad_norm(g)) == math.inf and float(hip.grad_norm(g, math.inf)) == torch.tensor(BIG).item()
+    out = [torch.full_like(t, 9.0) for t in g]
+    assert float(hip.clip_grads(hip.tensor_list(g, out=out), 1e38)) == math.inf and not any(bool(t.any()) for t in out)
+    p, m, v, step = new(), [torch.zeros_like(t) for t in g], [torch.zeros_like(t) for t in g], torch.zeros(2, device="cuda:0")
+    plan = hip.adam(p, g, m, v, step)
+    assert float(plan.run(0.1, max_norm=1e38)) == math.inf                                    # a share of 0: the step is taken with gradients of 0
+    assert all(torch.equal(a, b) for a, b in zip(p, new())) and not any(bool(t.any()) for t in m + v) and step.tolist() == [1.0, 1.0]
+    for given in (math.inf, math.nan, -math.inf):
+        assert not math.isfinite(float(plan.run(0.1, max_norm=1.0, grad_norm=torch.tensor(given, device="cuda:0"), skip_nonfinite=True)))
+        assert step.tolist() == [1.0, 1.0] and all(torch.equal(a, b) for a, b in zip(p, new()))
+    g[0][size // 2] = g[1][1] = 0.0
+    assert float(plan.run(0.1, max_norm=1.0, grad_norm=torch.tensor(4.0, device="cuda:0"), skip_nonfinite=True)) == 4.0 and step.tolist() == [2.0, 2.0]
+    g[0].fill_(0.0)
+    g[0][0], g[1][:] = 3.4e38, 0.0                                                                # the largest that are held
+    assert math.isfinite(float(hip.grad_norm(g))) and float(hip.clip_grads(g, 1.0)) == torch.tensor(3.4e38).item() and abs(float(g[0][0]) - 1.0) <= 2.0 ** -22
