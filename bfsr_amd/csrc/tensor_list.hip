@@ -229,7 +229,7 @@ __device__ __forceinline__ float share_of(const Norm& f, double norm)
 }
 
 struct Hyper { double lr, beta1, beta2, weight_decay; float eps; int decoupled, skip; const float* lr_at; };
-struct Factors { float size, root, keep, had; };               // of one row: lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), 1 - lr decay, the count before
+struct Factors { float size, root, decay, had; };              // of one row: lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), lr times the decay, the count before
 
 // b^t for a whole number t by squaring, in 64 bits (a count is at most 2^24, where float stops counting): 1 - b^t loses what 32 bits have for small t.
 __device__ __forceinline__ double power(double b, unsigned t)
@@ -244,7 +244,7 @@ __device__ __forceinline__ void begin_row(const Row& r, const Hyper& h, Factors*
     const float had = *r.step, t = had + 1.f;
     const double lr = h.lr_at ? (double)*h.lr_at : h.lr;
     *r.step = t;
-    *f = {(float)(lr / (1.0 - power(h.beta1, (unsigned)t))), (float)(1.0 / sqrt(1.0 - power(h.beta2, (unsigned)t))), (float)(1.0 - lr * h.weight_decay), had};
+    *f = {(float)(lr / (1.0 - power(h.beta1, (unsigned)t))), (float)(1.0 / sqrt(1.0 - power(h.beta2, (unsigned)t))), (float)(lr * h.weight_decay), had};
 }
 
 // A thread a row: 2.5 us for 8 rows, 4.8 for 702, which is three loads that depend on each other.
@@ -374,16 +374,17 @@ __global__ __launch_bounds__(TN) void clip_alone_kernel(const Row* __restrict__ 
     for (int c = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); c < count; c += TN / 64) clip_one<false>(rows, chunks[c], [=] { return s; });
 }
 
-struct Rule { float b1, c1, b2, c2, wd, eps; bool add, keep; Factors f; };
+struct Rule { float b1, c1, b2, c2, wd, eps; bool add, apart; Factors f; };
 
+// Decoupled decay goes into the update before that is taken off: 1 - lr decay has 24 bits, of which a small decay leaves few or none (of 1e-6 it made 1.013e-6, in every step).
 __device__ __forceinline__ void adam_element(const Rule& w, float share, float& p, float g, float& m, float& v)
 {
     float d = g * share;
     if (w.add) d = fmaf(w.wd, p, d);
-    if (w.keep) p *= w.f.keep;
     m = fmaf(w.b1, m, w.c1 * d);
     v = fmaf(w.b2, v, w.c2 * d * d);
-    p -= w.f.size * (m / fmaf(sqrtf(v), w.f.root, w.eps));
+    const float step = m / fmaf(sqrtf(v), w.f.root, w.eps);
+    p -= w.apart ? fmaf(w.f.size, step, w.f.decay * p) : w.f.size * step;
 }
 
 // One chunk for T threads; `share`: what its gradients are multiplied by, below 0 where the step is skipped.
@@ -437,7 +438,7 @@ __device__ __forceinline__ void adam_one(const Row* __restrict__ rows, const int
 {
     Rule w = {(float)h.beta1, (float)(1.0 - h.beta1), (float)h.beta2, (float)(1.0 - h.beta2), (float)h.weight_decay, h.eps};
     w.add = w.wd != 0.f && !h.decoupled;
-    w.keep = w.wd != 0.f && h.decoupled;
+    w.apart = w.wd != 0.f && h.decoupled;
     w.f = factors;
     const Row& r = rows[at.x];
     const long long begin = (long long)at.y * CHUNK;

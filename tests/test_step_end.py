@@ -307,7 +307,7 @@ def test_a_graph_captured_before_a_checkpoint_is_loaded():
         torch.cuda.synchronize()
         for p, s in zip(w, state):
             # steps of a constant gradient take the rate away: 0.25 by the ordinary step, none by the loaded rate of 0, 0.25 by each replay
-            assert float((p - (0.5 - 0.25 * k)).abs().max()) <= (16 * 2.0 ** -24 + 2e-8) * (k + 2)
+            assert float((p.detach() - (0.5 - 0.25 * k)).abs().max()) <= (16 * 2.0 ** -24 + 2e-8) * (k + 2)
             assert all(torch.equal(t, opt.state[p][n]) for n, t in s.items()) and float(s["step"]) == 8.0
     assert all(float(t.min()) == 7.0 == float(t.max()) for c in junk for t in c)
 
@@ -367,3 +367,19 @@ def test_norms_beyond_float32_are_infinite_everywhere(size):
     g[0].fill_(0.0)
     g[0][0], g[1][:] = 3.4e38, 0.0                                                                # the largest that are held
     assert math.isfinite(float(hip.grad_norm(g))) and float(hip.clip_grads(g, 1.0)) == torch.tensor(3.4e38).item() and abs(float(g[0][0]) - 1.0) <= 2.0 ** -22
+
+
+# ---- decoupled decay
+@gpu
+@pytest.mark.parametrize("lr, wd", [(1e-4, 1e-2), (1e-5, 1e-2), (1e-3, 0.1), (1e-2, 0.3)])
+@pytest.mark.parametrize("size", [2000, 70001])
+def test_small_decoupled_decay(size, lr, wd):
+    """Without gradients a step is the decay alone: (lr wd) p, rounded as a number of its own (its factor, the product and the update: 3 u of it) and off the parameter (u of that).
+    p times a rounded 1 - lr wd is off by up to half a u of p more, the same way for every p."""
+    hip = O.HipOps("cuda:0")
+    p = torch.randn(size, generator=torch.Generator().manual_seed(11)).cuda()
+    zeros = [torch.zeros_like(p) for _ in range(3)]
+    had, u = p.cpu().double(), 2.0 ** -24
+    hip.adam([p], zeros[:1], zeros[1:2], zeros[2:], torch.zeros(1, device="cuda:0")).run(lr, weight_decay=wd, decoupled=True)
+    want = had * (1 - lr * wd)
+    assert bool(((p.cpu().double() - want).abs() <= want.abs() * u + had.abs() * lr * wd * 3 * u + 2.0 ** -149).all())
