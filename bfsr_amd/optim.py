@@ -1,6 +1,6 @@
 """The end of a training step on the HIP kernels, for the modules that `linf/train.py` trains: gradient clipping by the global norm and Adam (the optimizer
 of LINF-LP/train.py:46-62).  Both take any list of dense float32 / float16 / bfloat16 parameters on one GPU in a few launches (ops.tensor_list, ops.adam),
-and neither waits for the device.
+and neither waits for the device; but the first step with a set of parameters that have gradients makes its table, and waits for the current stream once.
 
 `Adam` is a `torch.optim.Optimizer`: parameter groups, learning-rate schedulers and checkpoints work as with `torch.optim.Adam` / `AdamW`, whose
 state dicts it reads and whose state it writes (`step`, `exp_avg`, `exp_avg_sq`; moments are float32 whatever the parameter's type)."""
@@ -9,6 +9,7 @@ import torch
 from .ops import HipOps, _order
 
 _shared = {}
+PLANS = 4                  # sets of parameters with gradients that a group remembers (64 bytes of table a parameter each)
 
 
 def _ops_of(t, ops=None):
@@ -44,8 +45,8 @@ class Adam(torch.optim.Optimizer):
     max_grad_norm     clip the gradients of all groups by their global norm, within the update: p.grad is left as it is
     skip_nonfinite    a step whose gradients' norm is infinite or NaN changes nothing, step counts included
     `grad_norm` holds the last step's norm (0-d, on the device) where one of the two is asked for.
-    A group's lr may be a tensor of one float32 on the device; a step captured into a graph then follows it.  Capture after one ordinary step,
-    and again after load_state_dict: state and rate are new tensors then, and a graph goes on with the old ones, which it holds."""
+    A group's lr may be a tensor of one float32 on the device; a step captured into a graph then follows it.  Capture after one ordinary step with the
+    same parameters' gradients, and again after load_state_dict: state and rate are new tensors then, and a graph goes on with the old ones, which it holds."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled_weight_decay=False, max_grad_norm=None, skip_nonfinite=False,
                  ops=None):
@@ -110,27 +111,41 @@ class Adam(torch.optim.Optimizer):
                 self.state[p] = {"step": step, "exp_avg": self._moment(p), "exp_avg_sq": self._moment(p)}
         return [self.state[p] for p in params]
 
-    def _plan(self, at, ops, params, grads):
-        """The group's plan, if it still names the memory that parameters and state have, or a new one; the gradients in its order of axes, and where they are."""
-        state = self._state_of(params)
+    @staticmethod
+    def _where(params, state):
+        """The addresses of what a step writes."""
         where = [t.data_ptr() for t in params]
         for name in ("exp_avg", "exp_avg_sq", "step"):
             where += [s[name].data_ptr() for s in state]
-        held = self._plans.get(at)
-        if held is not None and (held[0] is not ops or held[1] != where):
-            held = None
-        found = None if held is None else held[2].fit(grads)
+        return where
+
+    def _fitting(self, at, ops, where, grads):
+        """A plan of the group that names this memory and takes these gradients, and where they are."""
+        for held in self._plans.get(at, ()):
+            if held[0] is ops and held[1] == where:
+                found = held[2].fit(grads)
+                if found is not None:
+                    return held[2], found
+        return None, None
+
+    def _plan(self, at, ops, params, grads):
+        """The group's plan of these parameters, if one still names the memory that they and their state have, or a new one; the gradients in its order of axes, and where they are."""
+        state = self._state_of(params)
+        where = self._where(params, state)
+        plan, found = self._fitting(at, ops, where, grads)
         if found is None:
             grads = [g if _order(g) == _order(p) and not g.is_neg() else torch.empty_like(p, dtype=g.dtype).copy_(g) for p, g in zip(params, grads)]
-            found = None if held is None else held[2].fit(grads)
+            plan, found = self._fitting(at, ops, where, grads)
         if found is None:
             bring = all(g.dtype == p.dtype for p, g in zip(params, grads))       # the plan holds no gradients, which zero_grad may want to free
             plan = ops.adam(params, None if bring else grads, *[[s[k] for s in state] for k in ("exp_avg", "exp_avg_sq", "step")])
-            held, found = (ops, where, plan), plan.fit(grads)
+            found = plan.fit(grads)
             if found is None:                        # without addresses the plan would go by its own column, which may be the parameters
                 raise ValueError("Adam: gradients that do not go with their parameters")
-            self._plans[at] = held
-        return held[2], grads, found
+            # older plans of other memory go: they hold what parameters and state were before
+            kept = [h for h in self._plans.get(at, ()) if all(self.state.get(p) for p in h[3]) and h[1] == self._where(h[3], [self.state[p] for p in h[3]])]
+            self._plans[at] = [(ops, where, plan, params)] + kept[:PLANS - 1]
+        return plan, grads, found
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -383,3 +383,95 @@ def test_small_decoupled_decay(size, lr, wd):
     hip.adam([p], zeros[:1], zeros[1:2], zeros[2:], torch.zeros(1, device="cuda:0")).run(lr, weight_decay=wd, decoupled=True)
     want = had * (1 - lr * wd)
     assert bool(((p.cpu().double() - want).abs() <= want.abs() * u + had.abs() * lr * wd * 3 * u + 2.0 ** -149).all())
+
+
+# ---- sets of parameters with gradients
+def test_alternating_sets_keep_their_plans(host):
+    """Conditional branches and partly frozen modules: each set's table is made once, and may be captured when it has been stepped with."""
+    w = [torch.nn.Parameter(torch.ones(n)) for n in (3, 4, 5)]
+    opt = optim.Adam([dict(params=w[:2]), dict(params=w[2:])], ops=host)
+
+    def step(which):
+        for k, p in enumerate(w):
+            p.grad = torch.ones_like(p) if k in which else None
+        opt.step()
+
+    for _ in range(3):
+        for which in ((0, 1, 2), (0,), (1, 2), (2,), ()):
+            step(which)
+    assert host.plans == 4                           # (0, 1), (0,) and (1,) of the first group, (2,) of the second
+    host.capturing = True
+    for which in ((0,), (1,), (0, 1, 2)):
+        step(which)
+    host.capturing = False
+    assert host.plans == 4
+    late = torch.nn.Parameter(torch.ones(2))
+    opt.add_param_group(dict(params=[late]))
+    late.grad = torch.ones(2)
+    host.capturing = True
+    with pytest.raises(RuntimeError):
+        opt.step()
+    host.capturing = False
+
+
+def test_plans_of_other_memory_are_let_go(host):
+    """A plan holds the parameters' and the state's memory: once they stand elsewhere it has to go, whichever set it was for."""
+    w = [torch.nn.Parameter(torch.ones(n)) for n in (3, 4)]
+    opt = optim.Adam(w, ops=host)
+
+    def step(which):
+        for k, p in enumerate(w):
+            p.grad = torch.ones_like(p) if k in which else None
+        opt.step()
+
+    step((0, 1))
+    step((0,))
+    before = refs([w[0].detach()] + [opt.state[w[0]][k] for k in ("exp_avg", "exp_avg_sq")])
+    w[0].data = torch.ones(3)
+    for k in ("exp_avg", "exp_avg_sq"):
+        opt.state[w[0]][k] = torch.zeros(3)
+    assert not any(r.expired() for r in before)
+    step((0,))
+    gc.collect()
+    assert all(r.expired() for r in before)
+    made = host.plans
+    step((0,))
+    assert host.plans == made
+    more = [torch.nn.Parameter(torch.ones(2)) for _ in range(4)]          # a few sets are remembered, not all
+    opt = optim.Adam(more, ops=host)
+    for bits in range(1, 16):
+        for k, p in enumerate(more):
+            p.grad = torch.ones_like(p) if bits >> k & 1 else None
+        opt.step()
+    assert len(opt._plans[0]) == optim.PLANS
+
+
+@gpu
+def test_alternating_sets_on_the_gpu():
+    """Against torch's Adam in 64 bits, the sets in turn and from a graph of one of them."""
+    hip = O.HipOps("cuda:0")
+    values = [torch.randn(n, generator=torch.Generator().manual_seed(n)) for n in (3, 3001, 5)]
+    own, ref = [torch.nn.Parameter(t.cuda()) for t in values], [torch.nn.Parameter(t.double()) for t in values]
+    opt, theirs = optim.Adam(own, lr=0.01, ops=hip), torch.optim.Adam(ref, lr=0.01)
+    static = [torch.zeros_like(p) for p in own]
+    graph, taken = None, 0
+    for k in range(8):
+        which = ((0, 1, 2), (0,), (1, 2))[k % 3]
+        for i, (a, b) in enumerate(zip(own, ref)):
+            g = torch.randn(b.shape, generator=torch.Generator().manual_seed(10 * k + i))
+            static[i].copy_(g)
+            a.grad, b.grad = (static[i], g.double()) if i in which else (None, None)
+        if k == 4:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                opt.step()
+        if graph is not None and k % 3 == 1:
+            graph.replay()
+        else:
+            opt.step()
+        theirs.step()
+        taken += 1
+        for a, b in zip(own, ref):
+            # each step's update is at most about 10 lr and off by a few dozen roundings of itself, and two of the parameter
+            assert bool(((a.detach().cpu().double() - b.detach()).abs() <= taken * 2.0 ** -24 * (4 * b.detach().abs() + 64 * 10 * 0.01)).all())
+    assert [float(opt.state[p]["step"]) for p in own] == [float(theirs.state[p]["step"]) for p in ref] and len(opt._plans[0]) == 3
