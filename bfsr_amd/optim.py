@@ -103,18 +103,21 @@ class Adam(torch.optim.Optimizer):
         return torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format, requires_grad=False)
 
     def _state_of(self, params):
-        new = [p for p in params if not self.state[p]]
-        if new:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("Adam: take an ordinary step before the capture begins (it makes the state)")
-            for p, step in zip(new, torch.zeros(len(new), dtype=torch.float32, device=new[0].device).unbind()):
-                self.state[p] = {"step": step, "exp_avg": self._moment(p), "exp_avg_sq": self._moment(p)}
+        state = [self.state[p] for p in params]
+        if all(state):
+            return state
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("Adam: take an ordinary step before the capture begins (it makes the state)")
+        new = [p for p, s in zip(params, state) if not s]
+        for p, step in zip(new, torch.zeros(len(new), dtype=torch.float32, device=new[0].device).unbind()):
+            self.state[p] = {"step": step, "exp_avg": self._moment(p), "exp_avg_sq": self._moment(p)}
         return [self.state[p] for p in params]
 
     @staticmethod
     def _where(params, state):
-        """The addresses of what a step writes."""
-        where = [t.data_ptr() for t in params]
+        """What tells the memory of a step: its addresses, and the parameters' orders of axes (set anew, one may be a transposed view of what it was)."""
+        where = [t.stride() for t in params]
+        where += [t.data_ptr() for t in params]
         for name in ("exp_avg", "exp_avg_sq", "step"):
             where += [s[name].data_ptr() for s in state]
         return where

@@ -475,3 +475,19 @@ def test_alternating_sets_on_the_gpu():
             # each step's update is at most about 10 lr and off by a few dozen roundings of itself, and two of the parameter
             assert bool(((a.detach().cpu().double() - b.detach()).abs() <= taken * 2.0 ** -24 * (4 * b.detach().abs() + 64 * 10 * 0.01)).all())
     assert [float(opt.state[p]["step"]) for p in own] == [float(theirs.state[p]["step"]) for p in ref] and len(opt._plans[0]) == 3
+
+
+def test_a_parameter_turned_in_its_memory(host):
+    """Same address, other order of the axes: the plan would pair its elements with others' gradients.  Its moments, in the old order, are refused; new ones go with it."""
+    w = torch.nn.Parameter(torch.ones(3, 3))
+    opt = optim.Adam([w], ops=host)
+    w.grad = torch.ones(3, 3)
+    opt.step()
+    w.data = w.data.t()
+    calls = len(host.lib.calls)
+    with pytest.raises(ValueError, match="strides"):
+        opt.step()
+    assert not [c for c in host.lib.calls[calls:] if c[0] == "bfsr_adam_step"]
+    opt.state.clear()
+    opt.step()
+    assert host.plans == 2 and opt.state[w]["exp_avg"].stride() == (1, 3)
