@@ -140,8 +140,9 @@ class Adam(torch.optim.Optimizer):
             grads = [g if _order(g) == _order(p) and not g.is_neg() else torch.empty_like(p, dtype=g.dtype).copy_(g) for p, g in zip(params, grads)]
             plan, found = self._fitting(at, ops, where, grads)
         if found is None:
-            bring = all(g.dtype == p.dtype for p, g in zip(params, grads))       # the plan holds no gradients, which zero_grad may want to free
+            bring = all(g.dtype == p.dtype for p, g in zip(params, grads))
             plan = ops.adam(params, None if bring else grads, *[[s[k] for s in state] for k in ("exp_avg", "exp_avg_sq", "step")])
+            plan.grads = None                        # every step brings its own: these are not held, since zero_grad may want to free them
             found = plan.fit(grads)
             if found is None:                        # without addresses the plan would go by its own column, which may be the parameters
                 raise ValueError("Adam: gradients that do not go with their parameters")

@@ -491,3 +491,21 @@ def test_a_parameter_turned_in_its_memory(host):
     opt.state.clear()
     opt.step()
     assert host.plans == 2 and opt.state[w]["exp_avg"].stride() == (1, 3)
+
+
+@pytest.mark.parametrize("types", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32)])
+def test_gradients_are_not_held(host, types):
+    """zero_grad frees them, whatever their type."""
+    w = torch.nn.Parameter(torch.ones(5, dtype=types[0]))
+    w.grad_dtype = types[1]
+    opt = optim.Adam([w], ops=host)
+    for _ in range(2):
+        w.grad = torch.ones(5, dtype=types[1])
+        ends = refs([w.grad])
+        opt.step()
+        opt.zero_grad()
+        gc.collect()
+        assert ends[0].expired()
+    assert host.plans == 1
+    with pytest.raises(ValueError):
+        opt._plans[0][0][2].run(0.1)                  # nor can the plan go by where they were
