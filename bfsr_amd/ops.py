@@ -288,8 +288,9 @@ def _at_least_0(v, what, below=math.inf):
 
 
 def _one_float(t, device, what):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device or t.layout is not torch.strided or t.is_neg():
         raise ValueError("%s: need a tensor of one float32 on %s" % (what, device))
+    _held(t, what)
     return t
 
 

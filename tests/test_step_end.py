@@ -509,3 +509,19 @@ def test_gradients_are_not_held(host, types):
     assert host.plans == 1
     with pytest.raises(ValueError):
         opt._plans[0][0][2].run(0.1)                  # nor can the plan go by where they were
+
+
+# ---- numbers on the device
+@pytest.mark.parametrize("bad", [lambda: conjugated(0.5), lambda: torch.ones(1).to_sparse(), lambda: freed((1,)), lambda: freed((), 8)])
+def test_numbers_on_the_device_are_real_memory(host, bad):
+    """A lazy minus sign would be lost, a freed rate would count as 0 or be read at an offset, a freed `out` be written there."""
+    p, g, m, v, step = make()
+    plan = host.adam(p, g, m, v, step)
+    t = bad()
+    for call in (lambda: plan.run(t), lambda: plan.run(0.1, max_norm=1.0, grad_norm=t), lambda: host.grad_norm(g, out=t), lambda: host.grad_norm([], out=t),
+                 lambda: host.adam(p[:1], g[:1], m[:1], v[:1], [t])):
+        with pytest.raises(ValueError):
+            call()
+    assert not [c for c in host.lib.calls if c[0] in ("bfsr_adam_step", "bfsr_grad_norm")]
+    plan.run(torch.tensor([0.5]), max_norm=1.0, grad_norm=torch.tensor(2.0))
+    assert [c[0] for c in host.lib.calls][-1] == "bfsr_adam_step"
