@@ -502,6 +502,8 @@ class HipOps(object):
         norm = self._norm_out(tensors, out)
         if tensors.n:
             tensors.call("grad_norm", self.lib.bfsr_grad_norm, kind, norm)
+            if out is not None and not out.is_inference():
+                torch.autograd.graph.increment_version(out)
         return norm
 
     def clip_grads(self, tensors, max_norm, norm_type=2.0):

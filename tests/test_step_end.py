@@ -525,3 +525,18 @@ def test_numbers_on_the_device_are_real_memory(host, bad):
     assert not [c for c in host.lib.calls if c[0] in ("bfsr_adam_step", "bfsr_grad_norm")]
     plan.run(torch.tensor([0.5]), max_norm=1.0, grad_norm=torch.tensor(2.0))
     assert [c[0] for c in host.lib.calls][-1] == "bfsr_adam_step"
+
+
+def test_a_norms_output_counts_as_changed(host):
+    """A backward pass that needs what `out` held before has to say so."""
+    g = make()[1]
+    for tensors in (g, host.tensor_list(g), []):
+        out = torch.ones(1)
+        x = torch.ones(1, requires_grad=True)
+        y = x * out
+        version = out._version
+        assert host.grad_norm(tensors, out=out) is out and out._version == version + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        host.grad_norm(g, out=torch.ones(()))
