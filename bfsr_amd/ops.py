@@ -251,14 +251,14 @@ class ListTable(object):
                 self.table.record_stream(torch.cuda.current_stream(i))
             if torch.cuda.is_current_stream_capturing():
                 _hold(ops.lib, stream, self, *reads)   # the table, and the memory that it names, whatever becomes of the list and its tensors
-        other, work = None, self.work
+        other, work, nbytes = None, self.work, self.bytes
         if grads is not None:
             other = torch.empty(self.n, dtype=torch.int64, device=self.device)
             _lib.check(ops.lib.bfsr_pointer_write(grads.ctypes.data, self.n, other.data_ptr(), stream), "pointer_write")
         if name == "grad_norm":
             own = torch.empty(self.norm_work, dtype=torch.float64, device=self.device) if self.norm_work else None
-            work = _ptr(own)
-        a = _lib.BfsrListArgs(self.rows, self.chunks, self.n, self.count, self.chunk, kind, _ptr(other), self.bytes, work, _ptr(norm))
+            work, nbytes = _ptr(own), self.read
+        a = _lib.BfsrListArgs(self.rows, self.chunks, self.n, self.count, self.chunk, kind, _ptr(other), nbytes, work, _ptr(norm))
         if ops._keylog is None and ops.profile_keys is None:
             err = fn(a, *more, stream)
         else:
@@ -315,7 +315,7 @@ class TensorList(ListTable):
             cols.append(_addresses(out, "tensor_list.out"))
             if Spans(cols[1], nbytes, "tensor_list.out").meet(at, nbytes):
                 raise ValueError("tensor_list.out: overlaps the tensors (leave `out` away to write in place)")
-        self.written = _versions(tensors if out is None else out)
+        self.written, self.read = _versions(tensors if out is None else out), int(nbytes.sum())      # a norm does not touch `out`
         sizes = np.array([t.numel() for t in tensors], dtype=np.int64)
         super().__init__(ops, cols, sizes, [LIST_TYPES[t.dtype] for t in tensors], nbytes.sum() * len(cols), once)
 

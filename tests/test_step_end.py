@@ -540,3 +540,13 @@ def test_a_norms_output_counts_as_changed(host):
             y.backward()
     with torch.inference_mode():
         host.grad_norm(g, out=torch.ones(()))
+
+
+def test_bytes_of_a_list_with_an_output(host):
+    """What a call touches decides whether it streams past the cache: a norm does not touch the output."""
+    g = make()[1]
+    total = sum(t.nbytes for t in g)
+    for tensors, whole in ((host.tensor_list(g), total), (host.tensor_list(g, out=[torch.zeros_like(t) for t in g]), 2 * total)):
+        host.grad_norm(tensors)
+        host.clip_grads(tensors, 1.0)
+        assert [args[0].bytes for name, args in host.lib.calls[-2:]] == [total, whole] and tensors.bytes == whole
