@@ -637,7 +637,7 @@ extern "C" int bfsr_clip_grads(const BfsrListArgs* a, float max_norm, void* stre
 extern "C" int bfsr_adam_step(const BfsrListArgs* a, const BfsrAdamArgs* h, void* stream)
 {
     if (!a || !h || !good(*a) || !a->work) return -1;
-    if (!(h->beta1 >= 0. && h->beta1 < 1.) || !(h->beta2 >= 0. && h->beta2 < 1.) || !(h->eps >= 0.f) || !(h->weight_decay >= 0.)) return -1;
+    if (!(h->beta1 >= 0. && h->beta1 < 1.) || !(h->beta2 >= 0. && h->beta2 < 1.) || !(h->eps >= 0.f) || !(h->weight_decay >= 0.) || h->max_norm != h->max_norm) return -1;
     hipStream_t st = (hipStream_t)stream;
     Factors* factors = (Factors*)((double*)a->work + PARTS);
     const bool norm = h->max_norm >= 0.f || h->skip_nonfinite, own = norm && !h->given_norm;

@@ -2,6 +2,7 @@
 
 `host` runs the host side of the operators on CPU tensors: the table, the checks and the calls as they are, without the kernels."""
 import contextlib
+import ctypes as C
 import gc
 import math
 import types
@@ -550,3 +551,12 @@ def test_bytes_of_a_list_with_an_output(host):
         host.grad_norm(tensors)
         host.clip_grads(tensors, 1.0)
         assert [args[0].bytes for name, args in host.lib.calls[-2:]] == [total, whole] and tensors.bytes == whole
+
+
+def test_a_bound_that_is_no_number_is_refused():
+    """... and not taken for `no clipping`, which any negative one is."""
+    lib = _lib.load()
+    a = _lib.BfsrListArgs(rows=4096, chunks=4096, n=1, count=1, chunk=lib.bfsr_list_chunk(1), work=4096, norm=4096)
+    for skip in (0, 1):
+        h = _lib.BfsrAdamArgs(beta1=0.9, beta2=0.999, max_norm=math.nan, skip_nonfinite=skip)
+        assert lib.bfsr_adam_step(C.byref(a), C.byref(h), None) == -1 == lib.bfsr_clip_grads(C.byref(a), math.nan, None)
