@@ -50,13 +50,26 @@ class Adam(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled_weight_decay=False, max_grad_norm=None, skip_nonfinite=False,
                  ops=None):
-        if not isinstance(lr, torch.Tensor) and not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0 or not all(0.0 <= b < 1.0 for b in betas):
-            raise ValueError("Adam: lr %r, eps %r, weight_decay %r or betas %r out of range" % (lr, eps, weight_decay, betas))
+        self._check(lr, betas, eps, weight_decay)
         if max_grad_norm is not None and not max_grad_norm >= 0.0:
             raise ValueError("Adam: max_grad_norm %r is out of range" % (max_grad_norm,))
         self.max_grad_norm, self.skip_nonfinite, self.grad_norm = max_grad_norm, skip_nonfinite, None
         self._ops, self._plans = ops, {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, decoupled_weight_decay=decoupled_weight_decay))
+
+    @staticmethod
+    def _check(lr, betas, eps, weight_decay):
+        if isinstance(lr, torch.Tensor):                 # its value now, where it can be waited for
+            ok = lr.numel() == 1 and (lr.is_cuda and torch.cuda.is_current_stream_capturing() or float(lr) >= 0.0)
+        else:
+            ok = lr >= 0.0
+        if not ok or not eps >= 0.0 or not weight_decay >= 0.0 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError("Adam: lr %r, eps %r, weight_decay %r or betas %r out of range" % (lr, eps, weight_decay, betas))
+
+    def add_param_group(self, param_group):
+        if isinstance(param_group, dict):
+            self._check(**{k: param_group.get(k, self.defaults[k]) for k in ("lr", "betas", "eps", "weight_decay")})
+        super().add_param_group(param_group)
 
     def __setstate__(self, state):
         super().__setstate__(state)

@@ -560,3 +560,19 @@ def test_a_bound_that_is_no_number_is_refused():
     for skip in (0, 1):
         h = _lib.BfsrAdamArgs(beta1=0.9, beta2=0.999, max_norm=math.nan, skip_nonfinite=skip)
         assert lib.bfsr_adam_step(C.byref(a), C.byref(h), None) == -1 == lib.bfsr_clip_grads(C.byref(a), math.nan, None)
+
+
+# ---- arguments of the optimizer
+@pytest.mark.parametrize("bad", [dict(lr=torch.tensor(-0.1)), dict(lr=torch.tensor(math.nan)), dict(lr=torch.tensor([0.1, 0.1])), dict(lr=-1.0), dict(eps=math.nan), dict(betas=(0.9, 1.0)),
+                                 dict(weight_decay=-1.0)])
+def test_groups_out_of_range_are_refused(bad):
+    w = [torch.nn.Parameter(torch.ones(3)) for _ in range(2)]
+    for make_it in (lambda: optim.Adam(w, **bad), lambda: optim.Adam([dict(params=w[:1]), dict(params=w[1:], **bad)])):
+        with pytest.raises(ValueError):
+            make_it()
+    opt = optim.Adam(w[:1], lr=torch.tensor(0.1))
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=w[1:], **bad))
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=w[1:], lr=torch.tensor([0.0]), eps=0.5))
+    assert [g["eps"] for g in opt.param_groups] == [1e-8, 0.5]
