@@ -27,11 +27,10 @@ def clip_grad_norm(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False
     """Scales the gradients of `parameters` (those that have one) in place so that their global norm (2 or inf) is at most `max_norm`; returns the norm before,
     a 0-d float32 tensor on the device.  error_if_nonfinite: waits for the norm and raises if it is infinite or NaN (the gradients are then scaled already:
     zero or NaN).  May be captured into a graph."""
-    if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
-        return torch.zeros(())
+        return torch.zeros((), device=parameters[0].device if parameters else None)
     ops = ops or _ops_of(grads[0])
     norm = ops.clip_grads(grads, max_norm, norm_type)
     if error_if_nonfinite and not torch.isfinite(norm):

@@ -576,3 +576,10 @@ def test_groups_out_of_range_are_refused(bad):
     assert len(opt.param_groups) == 1
     opt.add_param_group(dict(params=w[1:], lr=torch.tensor([0.0]), eps=0.5))
     assert [g["eps"] for g in opt.param_groups] == [1e-8, 0.5]
+
+
+def test_the_norm_of_no_gradients_is_on_their_device():
+    for w in (torch.nn.Parameter(torch.ones(3, device="meta")), [torch.nn.Parameter(torch.ones(3, device="meta"))], iter([torch.ones(3, device="meta")])):
+        norm = optim.clip_grad_norm(w, 1.0)
+        assert norm.device.type == "meta" and norm.shape == () and norm.dtype == torch.float32
+    assert float(optim.clip_grad_norm([], 1.0)) == 0.0
