@@ -143,12 +143,21 @@ class Adam(torch.optim.Optimizer):
                     return held[2], found
         return None, None
 
-    def _plan(self, at, ops, params, grads):
+    @staticmethod
+    def _refuse_sparse(grads):
+        if any(g.is_sparse for g in grads):
+            raise RuntimeError("Adam: sparse gradients are not supported")
+
+    def _plan(self, at, params, grads):
         """The group's plan of these parameters, if one still names the memory that they and their state have, or a new one; the gradients in its order of axes, and where they are."""
+        if at not in self._plans:
+            self._refuse_sparse(grads)
+        ops = self._ops or _ops_of(params[0])
         state = self._state_of(params)
         where = self._where(params, state)
         plan, found = self._fitting(at, ops, where, grads)
         if found is None:
+            self._refuse_sparse(grads)               # which no plan fits
             grads = [g if _order(g) == _order(p) and not g.is_neg() else torch.empty_like(p, dtype=g.dtype).copy_(g) for p, g in zip(params, grads)]
             plan, found = self._fitting(at, ops, where, grads)
         if found is None:
@@ -176,11 +185,8 @@ class Adam(torch.optim.Optimizer):
             if any(g is None for g in grads):
                 params = [p for p, g in zip(params, grads) if g is not None]
                 grads = [g for g in grads if g is not None]
-            if any(g.is_sparse for g in grads):
-                raise RuntimeError("Adam: sparse gradients are not supported")
             if params:
-                ops = self._ops or _ops_of(params[0])
-                work.append((group, *self._plan(at, ops, params, grads)))
+                work.append((group, *self._plan(at, params, grads)))
         self.grad_norm = None
         wants = self.max_grad_norm is not None or self.skip_nonfinite
         norm = None

@@ -583,3 +583,13 @@ def test_the_norm_of_no_gradients_is_on_their_device():
         norm = optim.clip_grad_norm(w, 1.0)
         assert norm.device.type == "meta" and norm.shape == () and norm.dtype == torch.float32
     assert float(optim.clip_grad_norm([], 1.0)) == 0.0
+
+
+def test_sparse_gradients_are_refused_at_every_step(host):
+    w = torch.nn.Parameter(torch.ones(3))
+    opt = optim.Adam([w], ops=host)
+    for g in (torch.ones(3).to_sparse(), torch.ones(3), torch.ones(3).to_sparse(), torch.ones(3)):
+        w.grad = g
+        with pytest.raises(RuntimeError, match="sparse") if g.is_sparse else contextlib.nullcontext():
+            opt.step()
+    assert [c[0] for c in host.lib.calls].count("bfsr_adam_step") == 2
