@@ -189,7 +189,7 @@ def _hold(lib, stream, table, *reads):
     ticket = C.c_void_p()
     _lib.check(lib.bfsr_capture_ticket(stream, C.byref(ticket)), "capture_ticket")
     with _captured_lock:
-        _captured.append((ticket.value, table, reads))
+        _captured.append((ticket.value, table, [t.detach() for t in reads]))
 
 
 def _let_go(lib):
@@ -389,16 +389,16 @@ class AdamPlan(ListTable):
 
     def _run(self, grads, lr, betas, eps, weight_decay, decoupled, max_norm, norm_type, grad_norm, skip_nonfinite):
         """run() with the addresses that fit() gave, or None."""
-        dev, at, reads = self.device, None, [t.detach() for t in (lr, grad_norm) if isinstance(t, torch.Tensor)]
+        dev, at, reads = self.device, None, ()
         if isinstance(lr, torch.Tensor):
-            at, lr = _one_float(lr, dev, "adam.lr").data_ptr(), 0.0
+            at, lr, reads = _one_float(lr, dev, "adam.lr").data_ptr(), 0.0, (lr,)
         beta1, beta2 = betas
         kind = _norm_type(norm_type)
         norm = given = None
         if max_norm is not None or skip_nonfinite:
             norm = torch.empty_like(self.scalar)
             if grad_norm is not None:
-                given = _one_float(grad_norm, dev, "adam.grad_norm").data_ptr()
+                given, reads = _one_float(grad_norm, dev, "adam.grad_norm").data_ptr(), reads + (grad_norm,)
         elif grad_norm is not None:
             raise ValueError("adam.grad_norm: goes with max_norm or skip_nonfinite")
         h = _lib.BfsrAdamArgs(_at_least_0(lr, "adam.lr"), at, _at_least_0(beta1, "adam.betas", 1.0), _at_least_0(beta2, "adam.betas", 1.0),
