@@ -240,7 +240,8 @@ class ListTable(object):
                 stream.synchronize()               # from here on the table may be read on any stream
 
     def call(self, name, fn, kind, norm, *more, grads=None, reads=()):
-        """One C call over the list on the current stream; `grads`: addresses in place of the table's gradients; `reads`: tensors that `more` names by their addresses."""
+        """One C call over the list on the current stream; `grads`: addresses in place of the table's gradients; `reads`: what else the call
+        knows by its address."""
         i = self.device.index
         if torch.cuda.current_device() != i:       # a launch needs its device to be the current one
             with torch.cuda.device(i):
@@ -501,7 +502,7 @@ class HipOps(object):
         kind, tensors = _norm_type(norm_type), self._listed(tensors)
         norm = self._norm_out(tensors, out)
         if tensors.n:
-            tensors.call("grad_norm", self.lib.bfsr_grad_norm, kind, norm)
+            tensors.call("grad_norm", self.lib.bfsr_grad_norm, kind, norm, reads=() if out is None else (out,))
             if out is not None and not out.is_inference():
                 torch.autograd.graph.increment_version(out)
         return norm

@@ -593,3 +593,18 @@ def test_sparse_gradients_are_refused_at_every_step(host):
         with pytest.raises(RuntimeError, match="sparse") if g.is_sparse else contextlib.nullcontext():
             opt.step()
     assert [c[0] for c in host.lib.calls].count("bfsr_adam_step") == 2
+
+
+def test_captured_norms_hold_their_output(host):
+    g, out = make()[1], torch.zeros(())
+    tensors = host.tensor_list(g)
+    ends = refs([out])
+    host.capturing = True
+    host.grad_norm(tensors, out=out)
+    host.capturing = False
+    del out
+    gc.collect()
+    assert not ends[0].expired()
+    host.lib.gone.add(1)
+    host.tensor_list(make()[1])
+    assert ends[0].expired()
