@@ -386,6 +386,9 @@ class AdamPlan(ListTable):
                 raise ValueError("adam.grads: need tensors of the plan's gradients' types, on its device, in the parameters' shapes and orders of axes")
         elif self.grads is None:
             raise ValueError("adam.grads: the plan was made without gradients, so run() needs them")
+        for t, what in ((lr, "adam.lr"), (grad_norm, "adam.grad_norm")):
+            if isinstance(t, torch.Tensor) and self.spans.meet(np.array([_one_float(t, self.device, what).data_ptr()]), np.array([4])):
+                raise ValueError("%s: is part of what the update writes" % what)
         return self._run(at, lr, betas, eps, weight_decay, decoupled, max_norm, norm_type, grad_norm, skip_nonfinite)
 
     def _run(self, grads, lr, betas, eps, weight_decay, decoupled, max_norm, norm_type, grad_norm, skip_nonfinite):

@@ -608,3 +608,14 @@ def test_captured_norms_hold_their_output(host):
     host.lib.gone.add(1)
     host.tensor_list(make()[1])
     assert ends[0].expired()
+
+
+def test_numbers_that_the_update_writes_are_refused(host):
+    """Some workgroups would read them before, some after."""
+    p, g, m, v, step = make()
+    plan = host.adam(p, g, m, v, step)
+    for t in (step[0], p[0][1], v[1][2, 1:2]):
+        for kw in (dict(lr=t), dict(lr=0.1, max_norm=1.0, grad_norm=t)):
+            with pytest.raises(ValueError, match="writes"):
+                plan.run(**kw)
+    plan.run(g[0][0], max_norm=1.0, grad_norm=g[1][0, 0])
