@@ -346,6 +346,7 @@ class AdamPlan(ListTable):
         self.grad_bytes = sizes * np.array([d.itemsize for d in grad_types])
         at = [_addresses(c, "adam." + name) for c, name in ((self.params, "params"), (self.exp_avg, "exp_avg"), (self.exp_avg_sq, "exp_avg_sq"), (self.step, "step"))]
         size = [_bytes(params), sizes * 4, sizes * 4, np.full_like(sizes, 4)]
+        self.counts = at[3]
         self.spans = Spans(np.concatenate(at), np.concatenate(size), "adam")
         grad_at = at[0] if grads is None else _addresses(self.grads, "adam.grads")
         if grads is not None and self.spans.meet(grad_at, self.grad_bytes):
@@ -386,9 +387,11 @@ class AdamPlan(ListTable):
                 raise ValueError("adam.grads: need tensors of the plan's gradients' types, on its device, in the parameters' shapes and orders of axes")
         elif self.grads is None:
             raise ValueError("adam.grads: the plan was made without gradients, so run() needs them")
-        for t, what in ((lr, "adam.lr"), (grad_norm, "adam.grad_norm")):
-            if isinstance(t, torch.Tensor) and self.spans.meet(np.array([_one_float(t, self.device, what).data_ptr()]), np.array([4])):
-                raise ValueError("%s: is part of what the update writes" % what)
+        # a rate is read when the counts are written, before the rest; a norm when the rest is
+        if isinstance(lr, torch.Tensor) and (self.counts == _one_float(lr, self.device, "adam.lr").data_ptr()).any():
+            raise ValueError("adam.lr: is a count that the update writes")
+        if isinstance(grad_norm, torch.Tensor) and self.spans.meet(np.array([_one_float(grad_norm, self.device, "adam.grad_norm").data_ptr()]), np.array([4])):
+            raise ValueError("adam.grad_norm: is part of what the update writes")
         return self._run(at, lr, betas, eps, weight_decay, decoupled, max_norm, norm_type, grad_norm, skip_nonfinite)
 
     def _run(self, grads, lr, betas, eps, weight_decay, decoupled, max_norm, norm_type, grad_norm, skip_nonfinite):
