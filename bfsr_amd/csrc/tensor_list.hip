@@ -1,4 +1,5 @@
-// tensor_list.hip -- the end of a training step over a LIST of tensors, in a few launches however many tensors the list has:
+// tensor_list.hip -- the end of a training step over a LIST of tensors, in one or two launches however many tensors the list has (and more where a call writes its table or brings
+// other gradients: one for each 149, 112 or 64 rows of one, two or five columns, one for each 480 addresses):
 //   bfsr_list_write / bfsr_pointer_write : the device table of a list (rows of pointers and sizes, and the chunks they are cut into)
 //   bfsr_grad_norm                       : global norm, sqrt(sum g^2) or max |g|
 //   bfsr_clip_grads                      : out = min(1, max_norm / (norm + 1e-6)) g
@@ -280,7 +281,8 @@ __device__ __forceinline__ double sum_chunks(const Row* __restrict__ rows, const
     return wave_join<MAX>((threadIdx.x & 63) < WAVES ? part[threadIdx.x & 63] : 0.0);
 }
 
-// Memory bounds it: 614 MB of fp32 in 93 us (6.6 TB/s, streaming), 77 MB of fp16 in 14 us (5.4), 18 MB in 6.0 us, where its start and end are most of it.
+// Memory bounds it: 614 MB of fp32 in 93 us (6.6 TB/s, streaming), 77 MB of fp16 in 14 us (5.4), 18 MB of fp32 in 6.0 us and 33 MB of bf16 in 9.8.  Of
+// those middle lists its start and end are a part, and idle CUs (2280 chunks at 16 a workgroup occupy 143 of them) and the rounds of a wave, one chunk after the other, are the rest.
 // One part of the norm for each of the first `sums` workgroups (with one, the norm itself); those behind them, if any, begin a step of Adam.
 template <bool MAX, bool STREAM>
 __global__ __launch_bounds__(TN) void norm_parts_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other,
@@ -451,7 +453,7 @@ __device__ __forceinline__ void adam_one(const Row* __restrict__ rows, const int
 __device__ __forceinline__ float share_of_step(const Norm& f, const Hyper& h, double norm) { return h.skip && !isfinite(norm) ? -1.f : share_of(f, norm); }
 
 // One chunk for each workgroup: two loads of 16 bytes from each of four arrays under way a thread, about fifty instructions an element, a division and a root among them.  Memory bounds
-// it: 153 M fp32 parameters (28 bytes each, none moved twice) in 705 us (6.1 TB/s), 16.7 M bf16 ones (22 bytes) in 62 us (5.9); 512 threads a chunk 2 % less to 2 % more.
+// it: 153 M fp32 parameters (28 bytes each, none moved twice) in 711 us (6.0 TB/s), 16.7 M bf16 ones (22 bytes) in 62 us (5.9); 512 threads a chunk 2 % less to 2 % more.
 // The workgroup behind the chunks sees to the norm's output, and to the counts of a step that is skipped.
 template <bool STREAM>
 __global__ __launch_bounds__(T) void adam_kernel(const Row* __restrict__ rows, const int2* __restrict__ chunks, const void* const* __restrict__ other, int count, int n,
@@ -496,7 +498,7 @@ __global__ __launch_bounds__(TN) void adam_alone_kernel(const Row* __restrict__ 
 }
 
 // ---- the table: rows and chunks travel to the device as kernel arguments.  No host buffer has to outlive the call, nothing waits for the stream, and a
-// captured graph holds what it needs.  A launch takes 149 rows (one column), 112 (two) or 64 (five) and 2.4 us.
+// captured graph of a table made in it holds what it needs.  A launch takes 149 rows (one column), 112 (two) or 64 (five) and 2.4 us.
 template <int COLS>
 struct Entry { const void* p[COLS]; long long n; int types, first; };          // first: the row's first chunk
 constexpr int ARGS = 3584;                                                     // bytes of a kernel's arguments that hold entries, of 4096

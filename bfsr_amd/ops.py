@@ -515,8 +515,8 @@ class HipOps(object):
 
     def clip_grads(self, tensors, max_norm, norm_type=2.0):
         """Multiplies a tensor_list, in place or into its `out`, or a plain list of tensors in place, by min(1, max_norm / (norm + 1e-6)); returns the norm
-        before (0-d float32, on the device).  An infinite norm (one beyond float32 is that, too) makes finite gradients 0, a NaN makes all NaN, as the quotient does.  Products are rounded
-        once, to the tensor's type.  What a graph is captured with stays allocated where it is a handle's; a plain list's tensors are the caller's to keep."""
+        before (0-d float32, on the device).  An infinite norm (one beyond float32 is that, too) makes finite gradients 0, a NaN makes all NaN, as the quotient does.  Products are formed in
+        32 bits, and rounded from those to a 16-bit type.  What a graph is captured with stays allocated where it is a handle's; a plain list's tensors are the caller's to keep."""
         kind, max_norm, tensors = _norm_type(norm_type), _at_least_0(max_norm, "clip_grads.max_norm"), self._listed(tensors)
         norm = self._norm_out(tensors, None)
         if tensors.n:

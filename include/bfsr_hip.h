@@ -604,7 +604,7 @@ int bfsr_to_uint8(const float* x, long long x_bs, unsigned char* y, int B, long 
  * bfsr_pointer_write: the same for a bare array of n pointers on the device (BfsrListArgs.other).
  *   bfsr_grad_norm : norm = sqrt(sum g^2), summed in 64 bits in an order fixed by the list (max: the largest |g|); NaN where an element is one.
  *   bfsr_clip_grads: out = g * min(1, max_norm / (norm + 1e-6)); `norm` gets the norm before it.
- *   bfsr_adam_step : t += 1; g *= share (max_norm >= 0); p *= 1 - lr wd (decoupled) or g += wd p; m = b1 m + (1 - b1) g; v = b2 v + (1 - b2) g^2;
+ *   bfsr_adam_step : t += 1; g *= share (max_norm >= 0; NaN is refused); p *= 1 - lr wd (decoupled) or g += wd p; m = b1 m + (1 - b1) g; v = b2 v + (1 - b2) g^2;
  *                    p -= lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps), in 32 bits, factors in 64, p rounded once to its type. */
 #define BFSR_LIST_ROW 64
 enum { BFSR_LIST_F32 = 0, BFSR_LIST_F16 = 1, BFSR_LIST_BF16 = 2 };
