@@ -496,7 +496,8 @@ class HipOps(object):
         axes and alignment, empty ones among them.  `out`: tensors of the same shapes, orders and types that take the clipped values (default: in place).
 
         The handle stands for the memory that the tensors have now, and holds it: their values are read at each call, but a gradient that is made anew (zero_grad
-        with set_to_none) needs a new handle, and so does one whose storage is resized.  Making one waits for the current stream; it may then be used on any
+        with set_to_none) needs a new handle, and so does one whose storage is resized.  Making one waits for the current stream (and for the device, once after a graph that held a handle has
+        gone); it may then be used on any
         stream, and in graphs, which have to be captured after it was made and hold the handle, and so that memory, as long as they exist.  Two calls that write the
         same tensors cannot run at the same time; norms can."""
         return TensorList(self, tensors, out)

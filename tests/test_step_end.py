@@ -619,3 +619,60 @@ def test_numbers_that_the_update_writes_are_refused(host):
             plan.run(**kw)
     plan.run(g[0][0], max_norm=1.0, grad_norm=g[1][0, 0])
     plan.run(p[0][0])                                               # a rate that is learned: read before the parameters are written
+
+
+# ---- calls in other surroundings
+@gpu
+def test_captured_step_of_two_groups_with_a_common_norm():
+    """Clipped by the norm over both groups, types mixed, against the same steps taken eagerly."""
+    hip = O.HipOps("cuda:0")
+    nets = []
+    for _ in range(2):
+        w = [torch.nn.Parameter(torch.randn(n, generator=torch.Generator().manual_seed(n)).cuda().to(t)) for n, t in ((70001, torch.float32), (3, torch.bfloat16), (5000, torch.bfloat16))]
+        w[2].grad_dtype = torch.float32
+        opt = optim.Adam([dict(params=w[:1]), dict(params=w[1:], lr=0.1)], lr=0.01, weight_decay=0.1, max_grad_norm=1.0, skip_nonfinite=True, ops=hip)
+        for p in w:
+            p.grad = torch.zeros_like(p, dtype=p.grad_dtype or p.dtype)
+        nets.append((w, opt))
+
+    def fill(k):
+        for w, _ in nets:
+            for i, p in enumerate(w):
+                p.grad.copy_(torch.randn(p.shape, generator=torch.Generator().manual_seed(100 * k + i)))
+
+    side = torch.cuda.Stream()
+    fill(0)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):                                   # ordinary steps on a stream of their own
+        for _, opt in nets:
+            opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        nets[0][1].step()
+    norm = nets[0][1].grad_norm
+    for k in range(1, 5):
+        fill(k)
+        if k == 3:
+            for w, _ in nets:
+                w[1].grad[1] = math.inf
+        graph.replay()
+        nets[1][1].step()
+        torch.cuda.synchronize()
+        assert float(norm) == float(nets[1][1].grad_norm) and math.isinf(float(norm)) == (k == 3)
+        for a, b in zip(nets[0][0], nets[1][0]):
+            assert torch.equal(a.detach(), b.detach())
+            assert all(torch.equal(nets[0][1].state[a][n], t) for n, t in nets[1][1].state[b].items())
+    assert [float(nets[0][1].state[p]["step"]) for p in nets[0][0]] == [4.0] * 3
+
+
+@gpu
+@pytest.mark.parametrize("size", [5, 70001])
+def test_a_learned_rate(size):
+    """One of the parameters is the rate: read before it is written."""
+    hip = O.HipOps("cuda:0")
+    p, g = [torch.full((1,), 0.25, device="cuda:0"), torch.full((size,), 1.0, device="cuda:0")], [torch.ones(1, device="cuda:0"), torch.ones(size, device="cuda:0")]
+    m, v, step = [torch.zeros_like(t) for t in p], [torch.zeros_like(t) for t in p], torch.zeros(2, device="cuda:0")
+    hip.adam(p, g, m, v, step).run(p[0], betas=(0.5, 0.5))
+    # the first step takes the rate away from all: within eps = 1e-8 of it, and a dozen roundings
+    assert abs(float(p[0])) <= 1e-8 + 16 * 2.0 ** -24 and float((p[1] - 0.75).abs().max()) <= 1e-8 + 16 * 2.0 ** -24
